@@ -333,7 +333,7 @@ def _plain_adamw(s):
     m = _of_8bit(s["first"], s["first_scale"]) if eight else s["first"]
     v = _of_8bit(s["second"], s["second_scale"]).square_() if eight else s["second"]
     m = m * a["beta1"] + g * (1 - a["beta1"])
-    v = v * a["beta2"] + g.square_() * (1 - a["beta2"])
+    v = v * a["beta2"] + g * g * (1 - a["beta2"])  # (g may be the gradient itself)
     del g
     root = v.sqrt()
     update = m / (1 - a["beta1"] ** s["step"]) / (root / math.sqrt(1 - a["beta2"] ** s["step"]) + a["eps"])
