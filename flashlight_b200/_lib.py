@@ -22,6 +22,7 @@ MATH_BY_NAME = {"strict": MATH_STRICT_F32, "tf32": MATH_TF32, "f32x3": MATH_F32X
 REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2
 ACT_NONE, ACT_GELU = 0, 1
 IDS_I32, IDS_I64 = 0, 1
+ADAMW_BLOCK = 256
 
 i32, i64, f32, f64, vp, sz = C.c_int32, C.c_int64, C.c_float, C.c_double, C.c_void_p, C.c_size_t
 
@@ -57,6 +58,15 @@ class RnnDesc(C.Structure):
     _fields_ = [(n, i32) for n in (
         "input_size", "hidden_size", "num_layers", "batch", "seq_len", "mode", "bidirectional",
         "dtype", "math_mode")]
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [(n, vp) for n in ("param", "grad", "first", "second", "first_scale", "second_scale")] + [("n", i64)]
+
+
+class AdamwDesc(C.Structure):
+    _fields_ = [(n, f64) for n in ("lr", "beta1", "beta2", "epsilon", "weight_decay", "grad_scale")] + [
+        ("step", i64), ("param_dtype", i32), ("grad_dtype", i32), ("state_bits", i32)]
 
 
 P = C.POINTER
@@ -140,6 +150,7 @@ SIGNATURES = {
     "flb200_attention_backward": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, f32,
                                             C.c_int, C.c_int, vp, sz, vp]),
     "flb200_sgd_step": (C.c_int, [vp, vp, vp, i64, f32, f32, f32, C.c_int, f32, C.c_int, C.c_int, vp]),
+    "flb200_adamw_step": (C.c_int, [P(AdamwDesc), P(AdamwTensor), i64, vp]),
     "flb200_relu_forward_mask": (C.c_int, [vp, vp, vp, i64, C.c_int, vp]),
     "flb200_relu_backward_mask": (C.c_int, [vp, vp, vp, i64, C.c_int, vp]),
     "flb200_add_relu_forward_mask": (C.c_int, [vp, vp, vp, vp, i64, C.c_int, vp]),

@@ -1,0 +1,321 @@
+// One AdamW step over many tensors at once (flb200_adamw_step):
+//     g = grad_scale * grad          m = beta1 m + (1 - beta1) g          v = beta2 v + (1 - beta2) g^2
+//     p = p - lr * (m / c1 / (sqrt(v / c2) + epsilon) + weight_decay * p),   c_i = 1 - beta_i^step
+// fl::AdamOptimizer::step (flashlight/fl/optim/AdamOptimizer.cpp) is the same moments as a chain of tensor
+// operators per parameter; a language model has a hundred and more parameters, most of them short.  Here the
+// tensors' addresses and lengths travel as the kernel's own argument, so that a step is one launch without a
+// table to copy first, and CTAs walk chunks of 2048 elements over all tensors.
+//
+// States of 8 bits: a warp owns a block of 256 elements.  m is kept as e4m3 times a scale per block (largest
+// magnitude / 448).  Of v its square root is kept, as e4m3 likewise: e4m3 spans a factor of 2^18 between its least
+// and its largest value, so v spans 2^36, and a relative error of at most 2^-4 of the root is one of the
+// step's length.  A root above zero is rounded up to the least code where it would become zero: it divides, and
+// m / epsilon would be a step a thousand times too long.  The step itself uses the new m and v before they are
+// rounded.  All arithmetic is in fp32; the step's quotient is the approximate one (2^-22 of its length, itself a
+// small part of p).
+//
+// HBM bounds it: 28 bytes per element in fp32, 10 with 16-bit parameters and gradients and 8-bit states.
+#include <cuda_fp8.h>
+
+#include <cmath>
+
+#include "common.cuh"
+
+namespace flb200 {
+namespace {
+
+constexpr int kPer = 8;                      // consecutive elements of a lane
+constexpr int kStateBlock = 32 * kPer;       // elements of a warp, and of a scale of 8-bit states
+constexpr int kChunk = 256 * kPer;           // elements of a CTA's pass
+static_assert(kStateBlock == FLB200_ADAMW_BLOCK, "a warp owns a block");
+
+struct AdamwMath {
+  float beta1, rest1, beta2, rest2;  // rest = 1 - beta
+  float inv_c1, inv_root_c2, epsilon, lr, weight_decay, grad_scale;
+};
+
+// Kernel arguments may take 32764 bytes; a launch copies what it is given, so short lists have short tables.
+template <int CAP>
+struct AdamwTable {
+  flb200_adamw_tensor t[CAP];
+  unsigned first_chunk[CAP + 1];  // chunks of the tensors before
+  unsigned vec[(CAP + 31) / 32];  // a bit per tensor: aligned for eight elements at once
+  int count;
+};
+constexpr int kSmall = 32, kMiddle = 160, kLarge = 480;
+static_assert(sizeof(AdamwTable<kLarge>) + sizeof(AdamwMath) < 32764, "kernel arguments");
+
+// Eight elements as fp32, of which `live` exist; whole: all do, and p is aligned to them.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool whole, int live, float* v) {
+  if (whole) {
+    if constexpr (sizeof(T) == 4) {
+      asm volatile("ld.global.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                   : "l"(p));
+    } else {
+      unpack16(load16(p), v);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) v[j] = j < live ? Num<T>::to_f(p[j]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, bool whole, int live, const float* v) {
+  if (whole) {
+    if constexpr (sizeof(T) == 4) {
+      asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]),
+                   "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                   : "memory");
+    } else {
+      store16(p, pack16<T>(v));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (j < live) p[j] = Num<T>::from_f(v[j]);
+  }
+}
+
+// Two fp32 numbers in one register pair: one instruction for both, each rounded as it would be alone.
+struct F2 {
+  unsigned long long r;
+};
+__device__ __forceinline__ F2 pair(float a, float b) {
+  F2 x;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x.r) : "f"(a), "f"(b));
+  return x;
+}
+__device__ __forceinline__ void unpair(F2 x, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.r));
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 x;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(x.r) : "l"(a.r), "l"(b.r));
+  return x;
+}
+// One by one: the assembler makes one rounding of a paired product and the paired sum behind it.
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  float a0, a1, b0, b1;
+  unpair(a, a0, a1);
+  unpair(b, b0, b1);
+  return pair(__fadd_rn(a0, b0), __fadd_rn(a1, b1));
+}
+__device__ __forceinline__ F2 fused(F2 a, F2 b, F2 c) {
+  F2 x;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x.r) : "l"(a.r), "l"(b.r), "l"(c.r));
+  return x;
+}
+
+// 8-bit states: eight codes, their values over the block's scale
+__device__ __forceinline__ void load_codes(const uint8_t* p, bool whole, int live, float scale, float* v) {
+  uint32_t w[2] = {0, 0};
+  if (whole) {
+    const uint2 c = *reinterpret_cast<const uint2*>(p);
+    w[0] = c.x;
+    w[1] = c.y;
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (j < live) w[j >> 2] |= (uint32_t)p[j] << (8 * (j & 3));
+  }
+  const F2 s = pair(scale, scale);
+#pragma unroll
+  for (int j = 0; j < kPer; j += 2) {
+    const __half2_raw h =
+        __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[j >> 2] >> (8 * (j & 2))), __NV_E4M3);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    unpair(pair(f.x, f.y) * s, v[j], v[j + 1]);
+  }
+}
+// The warp's block: its scale, and the codes of its values.  kRoot: values >= 0 of which none but zero becomes zero.
+template <bool kRoot>
+__device__ __forceinline__ void store_codes(uint8_t* p, float* scale, bool whole, int live, const float* v) {
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) top = fmaxf(top, kRoot ? v[j] : fabsf(v[j]));  // (past the end: zeros)
+  top = fmaxf(warp_max(top), 1e-30f);
+  const float to_code = __fmul_rn(__frcp_rn(top), 448.f);
+  const F2 k = pair(to_code, to_code);
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < kPer; j += 2) {
+    float2 s;
+    unpair(pair(v[j], v[j + 1]) * k, s.x, s.y);
+    if (kRoot) {
+      if (v[j] > 0.f) s.x = fmaxf(s.x, 0x1p-9f);
+      if (v[j + 1] > 0.f) s.y = fmaxf(s.y, 0x1p-9f);
+    }
+    const uint32_t two = __nv_cvt_float2_to_fp8x2(s, __NV_SATFINITE, __NV_E4M3);
+    w[j >> 2] |= two << (8 * (j & 2));
+  }
+  if (whole) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (j < live) p[j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+  }
+  if ((threadIdx.x & 31) == 0) *scale = __fmul_rn(top, 1.f / 448.f);
+}
+
+template <typename TP, typename TG, int BITS, int CAP>
+__global__ void __launch_bounds__(256)
+adamw_kernel(const __grid_constant__ AdamwTable<CAP> table, const AdamwMath k) {
+  chain_begin();
+  const unsigned chunks = table.first_chunk[table.count];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int at = 0;
+  for (unsigned chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+    // the last tensor that begins at or before this chunk (chunks of a CTA only grow)
+    int hi = table.count;
+    while (hi - at > 1) {
+      const int mid = (at + hi) >> 1;
+      if (table.first_chunk[mid] <= chunk) at = mid;
+      else hi = mid;
+    }
+    const flb200_adamw_tensor& t = table.t[at];
+    const long long block = (long long)(chunk - table.first_chunk[at]) * 8 + warp;  // of 256 elements
+    const long long i = block * kStateBlock + lane * kPer;
+    if (block * kStateBlock >= t.n) continue;  // (all lanes of the warp)
+    const long long left = t.n - i;
+    const int live = left >= kPer ? kPer : (left > 0 ? (int)left : 0);
+    const bool whole = live == kPer && (table.vec[at >> 5] >> (at & 31) & 1u);
+    float p[kPer], g[kPer], m[kPer], v[kPer];
+    load8(static_cast<const TP*>(t.param) + i, whole, live, p);
+    load8(static_cast<const TG*>(t.grad) + i, whole, live, g);
+    if constexpr (BITS == 32) {
+      load8(static_cast<const float*>(t.first) + i, whole, live, m);
+      load8(static_cast<const float*>(t.second) + i, whole, live, v);
+    } else {
+      load_codes(static_cast<const uint8_t*>(t.first) + i, whole, live, t.first_scale[block], m);
+      load_codes(static_cast<const uint8_t*>(t.second) + i, whole, live, t.second_scale[block], v);
+    }
+    // Each operation of the moments rounds by itself (no contraction): what is kept in 8 bits then depends on
+    // the formula alone.
+#pragma unroll
+    for (int j = 0; j < kPer; j += 2) {
+      const F2 gg = pair(g[j], g[j + 1]) * pair(k.grad_scale, k.grad_scale);
+      const F2 mm = pair(m[j], m[j + 1]) * pair(k.beta1, k.beta1) + gg * pair(k.rest1, k.rest1);
+      F2 vv = pair(v[j], v[j + 1]);
+      if (BITS == 8) vv = vv * vv;
+      vv = vv * pair(k.beta2, k.beta2) + gg * gg * pair(k.rest2, k.rest2);
+      float v0, v1, d0, d1, u0, u1;
+      unpair(vv, v0, v1);
+      const float r0 = __fsqrt_rn(v0), r1 = __fsqrt_rn(v1);
+      unpair(fused(pair(r0, r1), pair(k.inv_root_c2, k.inv_root_c2), pair(k.epsilon, k.epsilon)), d0, d1);
+      unpair(mm * pair(k.inv_c1, k.inv_c1), u0, u1);
+      const F2 pp = pair(p[j], p[j + 1]);
+      const F2 step = fused(pp, pair(k.weight_decay, k.weight_decay), pair(__fdividef(u0, d0), __fdividef(u1, d1)));
+      unpair(fused(step, pair(-k.lr, -k.lr), pp), p[j], p[j + 1]);
+      unpair(mm, m[j], m[j + 1]);
+      v[j] = BITS == 32 ? v0 : r0;
+      v[j + 1] = BITS == 32 ? v1 : r1;
+    }
+    store8(static_cast<TP*>(t.param) + i, whole, live, p);
+    if constexpr (BITS == 32) {
+      store8(static_cast<float*>(t.first) + i, whole, live, m);
+      store8(static_cast<float*>(t.second) + i, whole, live, v);
+    } else {
+      store_codes<false>(static_cast<uint8_t*>(t.first) + i, t.first_scale + block, whole, live, m);
+      store_codes<true>(static_cast<uint8_t*>(t.second) + i, t.second_scale + block, whole, live, v);
+    }
+  }
+}
+
+bool aligned_to(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+template <typename TP, typename TG, int BITS, int CAP>
+int launch_adamw(const AdamwMath& math, const flb200_adamw_tensor* tensors, int64_t* at, int64_t count,
+                 cudaStream_t st) {
+  AdamwTable<CAP> table;
+  table.count = 0;
+  table.first_chunk[0] = 0;
+  for (unsigned& w : table.vec) w = 0;
+  long long chunks = 0;
+  for (; *at < count && table.count < CAP; ++*at) {
+    const flb200_adamw_tensor& t = tensors[*at];
+    const long long mine = (t.n + kChunk - 1) / kChunk;
+    if (mine == 0) continue;
+    if (chunks + mine > 0x7fffffffLL) break;  // (one tensor alone has fewer, the entry point sees to it)
+    chunks += mine;
+    if (aligned_to(t.param, kPer * sizeof(TP)) && aligned_to(t.grad, kPer * sizeof(TG)) &&
+        aligned_to(t.first, kPer * BITS / 8) && aligned_to(t.second, kPer * BITS / 8))
+      table.vec[table.count >> 5] |= 1u << (table.count & 31);
+    table.t[table.count++] = t;
+    table.first_chunk[table.count] = (unsigned)chunks;
+  }
+  if (chunks == 0) return FLB200_OK;
+  const long long cap = 8LL * 4 * device_info().sm_count;
+  launch_chained(adamw_kernel<TP, TG, BITS, CAP>, (unsigned)(chunks < cap ? chunks : cap), 256, 0, st, table, math);
+  FLB200_AFTER_LAUNCH("adamw_step");
+  return FLB200_OK;
+}
+
+template <typename TP, typename TG, int BITS>
+int run_adamw(const AdamwMath& math, const flb200_adamw_tensor* tensors, int64_t count, cudaStream_t st) {
+  for (int64_t at = 0; at < count;) {
+    const int64_t left = count - at;
+    const int rc = left <= kSmall    ? launch_adamw<TP, TG, BITS, kSmall>(math, tensors, &at, count, st)
+                   : left <= kMiddle ? launch_adamw<TP, TG, BITS, kMiddle>(math, tensors, &at, count, st)
+                                     : launch_adamw<TP, TG, BITS, kLarge>(math, tensors, &at, count, st);
+    if (rc) return rc;
+  }
+  return FLB200_OK;
+}
+template <typename TP, typename TG>
+int run_adamw_bits(int bits, const AdamwMath& math, const flb200_adamw_tensor* tensors, int64_t count,
+                   cudaStream_t st) {
+  return bits == 32 ? run_adamw<TP, TG, 32>(math, tensors, count, st)
+                    : run_adamw<TP, TG, 8>(math, tensors, count, st);
+}
+
+}  // namespace
+}  // namespace flb200
+
+extern "C" int flb200_adamw_step(const flb200_adamw_desc* d, const flb200_adamw_tensor* tensors, int64_t count,
+                                 void* stream) {
+  using namespace flb200;
+  FLB200_REQUIRE(d && (tensors || count == 0) && count >= 0, "adamw_step: null argument");
+  FLB200_REQUIRE(d->step >= 1, "adamw_step: steps are counted from 1");
+  FLB200_REQUIRE(d->beta1 >= 0 && d->beta1 < 1 && d->beta2 >= 0 && d->beta2 < 1,
+                 "adamw_step: betas lie in [0, 1)");
+  FLB200_REQUIRE(d->epsilon >= 0, "adamw_step: negative epsilon");
+  FLB200_REQUIRE(d->state_bits == 32 || d->state_bits == 8, "adamw_step: states have 32 or 8 bits");
+  const int pt = d->param_dtype, gt = d->grad_dtype;
+  const bool half = pt == FLB200_F16 || pt == FLB200_BF16;
+  FLB200_REQUIRE(half || pt == FLB200_F32, "adamw_step: unknown dtype %d", pt);
+  FLB200_REQUIRE(gt == FLB200_F32 || gt == FLB200_F16 || gt == FLB200_BF16, "adamw_step: unknown dtype %d", gt);
+  if (half && gt != pt)
+    return fail(FLB200_UNSUPPORTED, "adamw_step: 16-bit parameters take gradients of their own type");
+  for (int64_t i = 0; i < count; ++i) {
+    const flb200_adamw_tensor& t = tensors[i];
+    FLB200_REQUIRE(t.n >= 0 && t.n <= (1LL << 40), "adamw_step: bad length");
+    if (t.n == 0) continue;
+    FLB200_REQUIRE(t.param && t.grad && t.first && t.second, "adamw_step: null tensor");
+    FLB200_REQUIRE(d->state_bits == 32 || (t.first_scale && t.second_scale),
+                   "adamw_step: 8-bit states need their scales");
+    const unsigned ps = half ? 2 : 4, gs = gt == FLB200_F32 ? 4 : 2, ss = d->state_bits / 8;
+    FLB200_REQUIRE(aligned_to(t.param, ps) && aligned_to(t.grad, gs) && aligned_to(t.first, ss) &&
+                       aligned_to(t.second, ss) && aligned_to(t.first_scale, 4) && aligned_to(t.second_scale, 4),
+                   "adamw_step: tensors must be aligned to their elements");
+  }
+  AdamwMath k;
+  k.beta1 = (float)d->beta1;
+  k.rest1 = (float)(1.0 - d->beta1);
+  k.beta2 = (float)d->beta2;
+  k.rest2 = (float)(1.0 - d->beta2);
+  k.inv_c1 = (float)(1.0 / (1.0 - std::pow(d->beta1, (double)d->step)));
+  k.inv_root_c2 = (float)(1.0 / std::sqrt(1.0 - std::pow(d->beta2, (double)d->step)));
+  k.epsilon = (float)d->epsilon;
+  k.lr = (float)d->lr;
+  k.weight_decay = (float)d->weight_decay;
+  k.grad_scale = (float)d->grad_scale;
+  const cudaStream_t st = as_stream(stream);
+  if (pt == FLB200_BF16) return run_adamw_bits<__nv_bfloat16, __nv_bfloat16>(d->state_bits, k, tensors, count, st);
+  if (pt == FLB200_F16) return run_adamw_bits<__half, __half>(d->state_bits, k, tensors, count, st);
+  if (gt == FLB200_BF16) return run_adamw_bits<float, __nv_bfloat16>(d->state_bits, k, tensors, count, st);
+  if (gt == FLB200_F16) return run_adamw_bits<float, __half>(d->state_bits, k, tensors, count, st);
+  return run_adamw_bits<float, float>(d->state_bits, k, tensors, count, st);
+}

@@ -14,6 +14,7 @@
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/Dtype.h>
@@ -24,6 +25,7 @@
 
 #include <cstdint>
 #include <initializer_list>
+#include <vector>
 
 #include "flb200.h"
 
@@ -925,6 +927,86 @@ NATIVE(batchnorm_add_relu_backward) {
   return wrap({gs, gx, gw, gb});
 }
 
+// ---------------------------------------------------------------- optimiser
+struct List {  // a Python list or tuple
+  PyObject* o;
+  Py_ssize_t n;
+  explicit List(PyObject* from) : o(from), n(0) {
+    if (!PyList_Check(o) && !PyTuple_Check(o)) {
+      PyErr_SetString(PyExc_TypeError, "expected a list or tuple of tensors");
+      throw PyRaised();
+    }
+    n = PySequence_Fast_GET_SIZE(o);
+  }
+  const Tensor* t(Py_ssize_t i) const {  // null for None
+    PyObject* v = PySequence_Fast_GET_ITEM(o, i);
+    if (v == Py_None) return nullptr;
+    if (!THPVariable_Check(v)) {
+      PyErr_SetString(PyExc_TypeError, "expected a tensor or None");
+      throw PyRaised();
+    }
+    return &THPVariable_Unpack(v);
+  }
+  const Tensor& tensor(Py_ssize_t i) const {
+    const Tensor* v = t(i);
+    if (!v) {
+      PyErr_SetString(PyExc_TypeError, "expected a tensor");
+      throw PyRaised();
+    }
+    return *v;
+  }
+};
+// (params, grads, firsts, seconds, first_scales or None, second_scales or None, step, lr, beta1, beta2, epsilon,
+//  weight_decay, grad_scale): parameters without a gradient are passed over; one launch per pair of types
+NATIVE(adamw_step) {
+  const List params(x.at(0)), grads(x.at(1)), firsts(x.at(2)), seconds(x.at(3));
+  const bool eight = x.at(4) != Py_None;
+  if (eight != (x.at(5) != Py_None)) value_error("adamw_step: 8-bit states need the scales of both moments");
+  const List s1(eight ? x.at(4) : x.at(0)), s2(eight ? x.at(5) : x.at(0));
+  for (const List* l : {&grads, &firsts, &seconds, &s1, &s2})
+    if (l->n != params.n) value_error("adamw_step: the lists must have one entry per parameter");
+  flb200_adamw_desc d = {};
+  d.step = x.i(6);
+  d.lr = x.d(7); d.beta1 = x.d(8); d.beta2 = x.d(9);
+  d.epsilon = x.d(10); d.weight_decay = x.d(11); d.grad_scale = x.d(12);
+  d.state_bits = eight ? 8 : 32;
+  const ScalarType state = eight ? ScalarType::Float8_e4m3fn : ScalarType::Float;
+  std::vector<flb200_adamw_tensor> group[3][3];
+  const int device = (int)c10::cuda::current_device();
+  for (Py_ssize_t i = 0; i < params.n; ++i) {
+    const Tensor& p = params.tensor(i);
+    const Tensor* g = grads.t(i);
+    if (!g) continue;
+    const Tensor &m = firsts.tensor(i), &v = seconds.tensor(i);
+    const int64_t n = p.numel();
+    if (!same_layout(p, *g)) value_error("adamw_step: a gradient must have its parameter's shape and layout");
+    if (m.numel() != n || v.numel() != n || m.scalar_type() != state || v.scalar_type() != state)
+      value_error("adamw_step: moments are float32, or float8_e4m3fn with scales, and as long as the parameter");
+    flb200_adamw_tensor t = {};
+    t.param = P(p); t.grad = P(*g); t.first = P(m); t.second = P(v); t.n = n;
+    if (eight) {
+      const Tensor &a = s1.tensor(i), &b = s2.tensor(i);
+      const int64_t blocks = (n + FLB200_ADAMW_BLOCK - 1) / FLB200_ADAMW_BLOCK;
+      if (a.numel() != blocks || b.numel() != blocks || a.scalar_type() != ScalarType::Float ||
+          b.scalar_type() != ScalarType::Float)
+        value_error("adamw_step: scales are float32, one per 256 elements");
+      t.first_scale = Pf(&a); t.second_scale = Pf(&b);
+    }
+    if (p.get_device() != device || g->get_device() != device || m.get_device() != device ||
+        v.get_device() != device)
+      value_error("adamw_step: tensors must be on the current device");
+    group[code_of(p)][code_of(*g)].push_back(t);
+  }
+  for (int pt = 0; pt < 3; ++pt)
+    for (int gt = 0; gt < 3; ++gt) {
+      const auto& ts = group[pt][gt];
+      if (ts.empty()) continue;
+      d.param_dtype = pt; d.grad_dtype = gt;
+      check(unlocked(flb200_adamw_step, (const flb200_adamw_desc*)&d, ts.data(), (int64_t)ts.size(), stream()));
+    }
+  Py_RETURN_NONE;
+}
+
 NATIVE(set_check) {  // (callable)
   Py_XDECREF(g_check);
   g_check = x.at(0);
@@ -934,7 +1016,7 @@ NATIVE(set_check) {  // (callable)
 
 #define ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
-    ENTRY(set_check), ENTRY(unary), ENTRY(binary), ENTRY(relu_mask), ENTRY(relu_mask_backward),
+    ENTRY(set_check), ENTRY(adamw_step), ENTRY(unary), ENTRY(binary), ENTRY(relu_mask), ENTRY(relu_mask_backward),
     ENTRY(dropout_apply), ENTRY(astype), ENTRY(reorder), ENTRY(bernoulli_mask), ENTRY(channel_sum),
     ENTRY(channel_bias_add), ENTRY(layernorm), ENTRY(layernorm_backward), ENTRY(linear),
     ENTRY(linear_bias_act), ENTRY(linear_backward), ENTRY(matmul), ENTRY(log_softmax),

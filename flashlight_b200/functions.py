@@ -260,6 +260,17 @@ def embedding_backward(grad_out, ids, vocab: int):
     return N.embedding_backward(grad_out.contiguous(), ids.contiguous(), vocab)
 
 
+# ------------------------------------------------------------------ optimiser
+def adamw_step(params, grads, firsts, seconds, *, step: int, lr: float, beta1: float = 0.9,
+               beta2: float = 0.999, eps: float = 1e-8, weight_decay: float = 0.0, grad_scale: float = 1.0,
+               first_scales=None, second_scales=None):
+    """One AdamW step (flb200_adamw_step) over lists of tensors, in place; `step` counts from 1.  A gradient of
+    None passes its parameter over.  firsts / seconds: m and v as float32; or, with the lists of their
+    scales (float32, one per L.ADAMW_BLOCK elements), m and sqrt(v) as float8_e4m3fn."""
+    N.adamw_step(params, grads, firsts, seconds, first_scales, second_scales, step, lr, beta1, beta2, eps,
+                 weight_decay, grad_scale)
+
+
 # ------------------------------------------------------------------ attention softmax
 def softmax(x, scale: float = 1.0, causal_period: int = 0):
     """softmax over the last dim of scale * x, optionally with the causal mask of stacked

@@ -1,4 +1,5 @@
-"""fl::SGDOptimizer (flashlight/fl/optim/SGDOptimizer.{h,cpp}) over the fused step kernel."""
+"""fl::SGDOptimizer (flashlight/fl/optim/SGDOptimizer.{h,cpp}) over the fused step kernel, and AdamW over all
+parameters at once."""
 from __future__ import annotations
 
 from typing import List
@@ -6,6 +7,7 @@ from typing import List
 import torch
 
 from . import _lib as L
+from . import functions as F
 from .autograd import Variable
 from .extension import ptr, stream_handle
 
@@ -34,6 +36,57 @@ class SGDOptimizer:
             L.check(L.lib.flb200_sgd_step(ptr(p.tensor), ptr(g), ptr(v), p.tensor.numel(), self.lr,
                                           self.mu, self.wd, 1 if self.nesterov else 0, grad_scale,
                                           1 if zero_grad else 0, L.F32, stream_handle()))
+
+    def zeroGrad(self) -> None:
+        for p in self.parameters:
+            p.zeroGrad()
+
+
+class AdamWOptimizer:
+    """The moments of fl::AdamOptimizer (flashlight/fl/optim/AdamOptimizer.{h,cpp}) with the weight decay beside
+    the step: p -= lr * (m^ / (sqrt(v^) + epsilon) + weight_decay * p).  One launch for all parameters
+    (functions.adamw_step).  state_bits=8 keeps m and sqrt(v) as e4m3 bytes with a scale per 256 elements:
+    2 bytes per element instead of 8.  Parameters without a gradient are passed over; the step's number counts
+    all calls.  The states of all parameters lie one after another in `first` and `second`."""
+
+    def __init__(self, parameters: List[Variable], learning_rate: float, beta1: float = 0.9,
+                 beta2: float = 0.999, epsilon: float = 1e-8, weight_decay: float = 0.0, state_bits: int = 32):
+        if state_bits not in (32, 8):
+            raise ValueError("AdamWOptimizer: states have 32 or 8 bits")
+        self.parameters = list(parameters)
+        self.lr, self.beta1, self.beta2 = learning_rate, beta1, beta2
+        self.eps, self.wd, self.state_bits, self.steps = epsilon, weight_decay, state_bits, 0
+        tensors = [p.tensor for p in self.parameters]
+        if not all(t.is_contiguous() for t in tensors):
+            raise ValueError("AdamWOptimizer: parameters must be contiguous")
+        blocks = [(t.numel() + L.ADAMW_BLOCK - 1) // L.ADAMW_BLOCK for t in tensors]
+        self.first, self.firsts = self._states(tensors, blocks)
+        self.second, self.seconds = self._states(tensors, blocks)
+        self.first_scale = self.second_scale = self.first_scales = self.second_scales = None
+        if state_bits == 8:
+            device = self.first.device
+            self.first_scale, self.second_scale = (torch.zeros(sum(blocks), device=device) for _ in range(2))
+            self.first_scales, self.second_scales = self.first_scale.split(blocks), self.second_scale.split(blocks)
+
+    def _states(self, tensors, blocks):
+        """Zeros for all parameters in one buffer, each parameter on blocks of its own, and its part of them."""
+        device = tensors[0].device if tensors else "cuda"
+        eight = self.state_bits == 8
+        buffer = torch.zeros(sum(blocks) * L.ADAMW_BLOCK, dtype=torch.uint8 if eight else torch.float32,
+                             device=device)
+        if eight:
+            buffer = buffer.view(torch.float8_e4m3fn)
+        parts = buffer.split([n * L.ADAMW_BLOCK for n in blocks])
+        return buffer, [part[:t.numel()] for part, t in zip(parts, tensors)]
+
+    def step(self, grad_scale: float = 1.0) -> None:
+        self.steps += 1
+        grads = [p.grad for p in self.parameters]
+        F.adamw_step([p.tensor for p in self.parameters],
+                     [g if g is None or g.is_contiguous() else g.contiguous() for g in grads], self.firsts,
+                     self.seconds, step=self.steps, lr=self.lr, beta1=self.beta1, beta2=self.beta2, eps=self.eps,
+                     weight_decay=self.wd, grad_scale=grad_scale, first_scales=self.first_scales,
+                     second_scales=self.second_scales)
 
     def zeroGrad(self) -> None:
         for p in self.parameters:

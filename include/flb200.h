@@ -503,6 +503,38 @@ int flb200_sgd_step(void* param, void* grad, void* velocity, int64_t n, float lr
                     float weight_decay, int nesterov, float grad_scale, int zero_grad, int dtype,
                     void* stream);
 
+/* One AdamW step over `count` tensors in one launch per 480 of them: the moments of fl::AdamOptimizer
+ * (flashlight/fl/optim/AdamOptimizer.cpp) with the weight decay beside the step:
+ *   g = grad_scale * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   p = p - lr * (m / (1 - beta1^step) / (sqrt(v / (1 - beta2^step)) + epsilon) + weight_decay * p)
+ * `step` counts from 1.  All arithmetic is in fp32.  param_dtype f32 with gradients of any type, or a
+ * 16-bit type with gradients of that type (else FLB200_UNSUPPORTED).
+ * state_bits 32: first = m and second = v in f32; the scales are not used.
+ * state_bits 8: blocks of FLB200_ADAMW_BLOCK elements, the last one of a tensor may be short:
+ *   first  = m / first_scale[block] and second = sqrt(v) / second_scale[block] as e4m3 bytes, a scale being
+ *   the block's largest magnitude / 448; a root above zero has a code above zero.  The step uses m and v
+ *   before they are rounded.  An infinite gradient leaves NaN in its whole block's states.
+ * Tensors aligned to eight elements (of f32: 32 bytes) are read in whole vectors, others one by one.  Empty
+ * tensors are passed over.  Everything is read on the host during the call: `tensors` may be reused after it. */
+enum { FLB200_ADAMW_BLOCK = 256 };
+typedef struct flb200_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* first;
+  void* second;
+  float* first_scale;   /* [ceil(n / 256)], state_bits 8 */
+  float* second_scale;
+  int64_t n;
+} flb200_adamw_tensor;
+typedef struct flb200_adamw_desc {
+  double lr, beta1, beta2, epsilon, weight_decay, grad_scale;
+  int64_t step;
+  int32_t param_dtype, grad_dtype;
+  int32_t state_bits;
+} flb200_adamw_desc;
+int flb200_adamw_step(const flb200_adamw_desc* d, const flb200_adamw_tensor* tensors, int64_t count,
+                      void* stream);
+
 /* fl::embedding (Functions.cpp:1707-1749): out row r = table row ids[r]; table [vocab][dim]
  * row-major (fl [dim, vocab]), ids int32 or int64, out [rows][dim].  Ids outside [0, vocab)
  * give a zero row / are ignored by the gradient. */
