@@ -69,6 +69,11 @@ class AdamwDesc(C.Structure):
         ("step", i64), ("param_dtype", i32), ("grad_dtype", i32), ("state_bits", i32)]
 
 
+class LinearCceDesc(C.Structure):
+    _fields_ = [("rows", i64), ("features", i64), ("classes", i64), ("reduction", i32), ("ignore_index", i32),
+                ("dtype", i32)]
+
+
 P = C.POINTER
 # name -> (restype, argtypes); one entry per declaration in include/flb200.h
 SIGNATURES = {
@@ -182,6 +187,11 @@ SIGNATURES = {
                                             sz, vp]),
     "flb200_scores_cce_backward": (C.c_int, [vp, vp, vp, vp, vp, vp, i64, i64, C.c_int, C.c_int, C.c_int,
                                              vp]),
+    "flb200_linear_cce_supported": (C.c_int, [P(LinearCceDesc)]),
+    "flb200_linear_cce_workspace_bytes": (sz, [P(LinearCceDesc), vp, vp, C.c_int]),
+    "flb200_linear_cce_forward": (C.c_int, [P(LinearCceDesc), vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "flb200_linear_cce_backward": (C.c_int, [P(LinearCceDesc), vp, vp, vp, vp, vp, vp, vp, vp, vp, C.c_int, vp,
+                                             vp, sz, vp]),
     "flb200_rnn_num_params": (i64, [P(RnnDesc)]),
     "flb200_rnn_reserve_bytes": (sz, [P(RnnDesc)]),
     "flb200_rnn_workspace_bytes": (sz, [P(RnnDesc), C.c_int]),

@@ -578,6 +578,30 @@ def log_softmax_cross_entropy(x: Variable, targets: torch.Tensor, reduction=L.RE
     return Variable(loss, False, [x], grad_func)
 
 
+def linear_cross_entropy(x: Variable, w: Variable, b: Optional[Variable], targets: torch.Tensor,
+                         reduction=L.REDUCE_MEAN, ignore_index=-1) -> Variable:
+    """log_softmax_cross_entropy(linear(x, w, b), targets) of f16 / bf16 tensors without the scores or their
+    gradient in memory: of the forward pass each row's log-sum-exp is kept, and the gradient makes the scores again,
+    a piece of the vocabulary at a time.  Other tensors take the operators one by one."""
+    xt, wt, bt = x.tensor.contiguous(), w.tensor.contiguous(), b.tensor if b is not None else None
+    fused = None
+    if xt.dtype in (torch.float16, torch.bfloat16) and wt.dtype == xt.dtype:
+        fused = F.linear_cross_entropy(xt, wt, bt, targets, reduction, ignore_index)
+    if fused is None:
+        return log_softmax_cross_entropy(linear(x, w, b), targets, reduction, ignore_index, wide=True)
+    loss, state, lse = fused
+
+    def grad_func(inputs, gl):
+        need = [i.isCalcGrad() for i in inputs] + [False]
+        grads = F.linear_cross_entropy_backward(xt, wt, bt, lse, gl.contiguous(), state, need[0], need[1], need[2],
+                                                wide=w.grad_dtype == torch.float32)
+        for inp, g in zip(inputs, grads):
+            if g is not None:
+                inp.addGrad(_as(g, inp.tensor.shape))
+
+    return Variable(loss, False, [x, w] + ([b] if b is not None else []), grad_func)
+
+
 # ------------------------------------------------ pieces of the Transformer workload
 def glue(x: Variable, fwd, bwd) -> Variable:
     """A data-movement step that has no kernel in this library (permutations between the

@@ -927,6 +927,59 @@ NATIVE(batchnorm_add_relu_backward) {
   return wrap({gs, gx, gw, gb});
 }
 
+// linear + logSoftmax + cross entropy without the scores
+flb200_linear_cce_desc linear_cce_desc(const Tensor& in, const Tensor& w, const Tensor* bias, const Tensor& targets,
+                                       int reduction, int ignore) {
+  const LinearDims l = linear_dims(w, in);
+  if (targets.numel() != l.cols) value_error("dimension mismatch in categorical cross entropy");
+  if (targets.scalar_type() != ScalarType::Int) value_error("linear_cross_entropy: targets are int32");
+  if (w.dim() != 2 || w.scalar_type() != in.scalar_type())
+    value_error("linear_cross_entropy: input and weight must be of one type");
+  if (bias && (bias->numel() != l.O || bias->scalar_type() != ScalarType::Float))
+    value_error("linear_cross_entropy: the bias is float32, one per class");
+  flb200_linear_cce_desc d = {};
+  d.rows = l.cols; d.features = l.I; d.classes = l.O;
+  d.reduction = reduction; d.ignore_index = ignore; d.dtype = code_of(in);
+  return d;
+}
+// (x, weight, bias or None, targets int32, reduction, ignore_index) -> (loss, meta, lse), or None where the
+// library has no kernel for the tensors
+NATIVE(linear_cce_forward) {
+  const Tensor &in = x.tensor(0), &w = x.tensor(1), &tg = x.tensor(3);
+  const Tensor* bias = x.t(2);
+  const flb200_linear_cce_desc d = linear_cce_desc(in, w, bias, tg, x.n32(4), x.n32(5));
+  if (d.rows < 1 || !in.is_contiguous() || !w.is_contiguous() || !flb200_linear_cce_supported(&d)) Py_RETURN_NONE;
+  Tensor loss = floats(d.reduction == FLB200_REDUCE_NONE ? d.rows : 1, in), lse = floats(d.rows, in);
+  Tensor meta = empty({2}, ScalarType::Int, in);  // [count, bad-target flag]
+  int32_t* m = static_cast<int32_t*>(meta.data_ptr());
+  void* st = stream();
+  if (unlocked(cudaMemsetAsync, m, 0, (size_t)8, static_cast<cudaStream_t>(st)) != cudaSuccess)
+    check(FLB200_LAUNCH_FAILURE);
+  Workspace ws(flb200_linear_cce_workspace_bytes(&d, P(in), P(w), 0), in);
+  check(unlocked(flb200_linear_cce_forward, &d, P(in), P(w), Pf(bias), static_cast<const int32_t*>(P(tg)), Pf(&loss),
+                 Pf(&lse), m, m + 1, ws.p(), ws.bytes, st));
+  return wrap({loss, meta, lse});
+}
+// (x, weight, bias or None, lse, grad_loss, targets, meta, reduction, ignore_index, need_x, need_w, need_b, wide)
+//   -> (grad_x, grad_w, grad_b)
+NATIVE(linear_cce_backward) {
+  const Tensor &in = x.tensor(0), &w = x.tensor(1), &gl = x.tensor(4), &tg = x.tensor(5), &meta = x.tensor(6);
+  const Tensor* bias = x.t(2);
+  const flb200_linear_cce_desc d = linear_cce_desc(in, w, bias, tg, x.n32(7), x.n32(8));
+  if (gl.numel() != (d.reduction == FLB200_REDUCE_NONE ? d.rows : 1) || gl.scalar_type() != ScalarType::Float)
+    value_error("linear_cross_entropy: the loss's gradient must be float32 and of the loss's shape");
+  Tensor gx, gw, gb;
+  if (x.b(9)) gx = empty_like(in);
+  if (x.b(10)) gw = empty(w.sizes(), x.b(12) ? ScalarType::Float : w.scalar_type(), w);
+  if (x.b(11)) gb = floats(d.classes, in);
+  Workspace ws(flb200_linear_cce_workspace_bytes(&d, P(in), P(w), 1), in);
+  check(unlocked(flb200_linear_cce_backward, &d, P(in), P(w), Pf(bias), Pf(x.t(3)), Pf(&gl),
+                 static_cast<const int32_t*>(P(tg)), static_cast<const int32_t*>(P(meta)),
+                 gx.defined() ? P(gx) : nullptr, gw.defined() ? P(gw) : nullptr,
+                 gw.defined() ? code_of(gw) : d.dtype, gb.defined() ? Pf(&gb) : nullptr, ws.p(), ws.bytes, stream()));
+  return wrap({gx, gw, gb});
+}
+
 // ---------------------------------------------------------------- optimiser
 struct List {  // a Python list or tuple
   PyObject* o;
@@ -1016,7 +1069,7 @@ NATIVE(set_check) {  // (callable)
 
 #define ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
-    ENTRY(set_check), ENTRY(adamw_step), ENTRY(unary), ENTRY(binary), ENTRY(relu_mask), ENTRY(relu_mask_backward),
+    ENTRY(set_check), ENTRY(adamw_step), ENTRY(linear_cce_forward), ENTRY(linear_cce_backward), ENTRY(unary), ENTRY(binary), ENTRY(relu_mask), ENTRY(relu_mask_backward),
     ENTRY(dropout_apply), ENTRY(astype), ENTRY(reorder), ENTRY(bernoulli_mask), ENTRY(channel_sum),
     ENTRY(channel_bias_add), ENTRY(layernorm), ENTRY(layernorm_backward), ENTRY(linear),
     ENTRY(linear_bias_act), ENTRY(linear_backward), ENTRY(matmul), ENTRY(log_softmax),

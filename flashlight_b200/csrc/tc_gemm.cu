@@ -531,6 +531,11 @@ int build_operand(const Side& s, const void* base, long long rows, long long K, 
 
 }  // namespace
 
+int tc::matrix_operand(bool mn_major, long long ld, const void* base, long long rows, long long K, int tile_rows,
+                       int operand, CUtensorMap* map, OperandPlan* plan) {
+  return build_operand(Side{true, mn_major, ld}, base, rows, K, 1, 0, tile_rows, map, plan, operand);
+}
+
 bool tc_gemm_supported(const flb200_matmul_desc* d, const void* a, const void* b, const void* c) {
   if (device_info().cc_major != 10) return false;
   if (!tc::encode_tiled_fn()) return false;

@@ -138,6 +138,12 @@ struct X3Scope {
 int* status_ptr();
 void count_tc_launch();
 
+// Tensor map and plan of a matrix operand op(r, k) of rows x K elements: K-major, at base[r * ld + k], or
+// MN-major, at base[k * ld + r]; `tile_rows` rows per stage (kBM, or Launch::b_box_rows()).  base and rows of ld
+// elements are 16-byte aligned.
+int matrix_operand(bool mn_major, long long ld, const void* base, long long rows, long long K, int tile_rows,
+                   int operand, CUtensorMap* map, OperandPlan* plan);
+
 // Launches the contraction as planned (and the split-K reduction when the plan splits K).  With
 // less scratch than the plan wants, fewer splits run; with none, one.
 int run(const CUtensorMap& ma, const CUtensorMap& mb, const OperandPlan& pa, const OperandPlan& pb,

@@ -249,6 +249,25 @@ def scores_cross_entropy_backward(x, lse, grad_loss, state: CrossEntropyState):
                                  state.ignore_index)
 
 
+def linear_cross_entropy(x, weight, bias, targets, reduction: int = L.REDUCE_MEAN, ignore_index: int = -1):
+    """categoricalCrossEntropy(logSoftmax(linear(x))) without the scores in memory (f16 and bf16 tensors; bias
+    float32 or None).  Returns (loss, state, lse), or None where the library has no kernel for the tensors."""
+    if targets.dtype != torch.int32:
+        targets = targets.to(torch.int32)
+    out = N.linear_cce_forward(x, weight, bias, targets, reduction, ignore_index)
+    if out is None:
+        return None
+    return out[0], CrossEntropyState(targets, out[1], reduction, ignore_index), out[2]
+
+
+def linear_cross_entropy_backward(x, weight, bias, lse, grad_loss, state: CrossEntropyState, need_input_grad=True,
+                                  need_weight_grad=True, need_bias_grad=True, wide: bool = False):
+    """Returns (grad_x, grad_weight, grad_bias), None for those not asked for; wide: grad_weight in float32."""
+    return N.linear_cce_backward(x, weight, bias, lse, grad_loss, state.targets, state.count, state.reduction,
+                                 state.ignore_index, need_input_grad, need_weight_grad,
+                                 bias is not None and need_bias_grad, wide)
+
+
 # ------------------------------------------------------------------ embedding
 def embedding(table, ids):
     """fl::embedding forward: rows of `table` (vocab, dim) picked by `ids` (any shape)."""

@@ -637,6 +637,34 @@ int flb200_scores_cce_backward(const void* x, const float* lse, const float* gra
                                int64_t C, int64_t X, int reduction, int ignore_index, int dtype,
                                void* stream);
 
+/* categoricalCrossEntropy(logSoftmax(linear(x))) (Functions.cpp:1255-1309, 1044-1154) for a large vocabulary,
+ * without the scores: x [features, rows], weight [classes, features] as in flb200_linear_forward (row-major
+ * [rows][features] and [features][classes]), bias fp32 or NULL, targets int32 [rows].  Forward keeps lse [rows],
+ * the log of the sum of each row's exponentials; backward makes the scores again, a piece of the vocabulary at a
+ * time.  FLB200_F16 or FLB200_BF16 tensors, any extents and alignment; scores, statistics and sums in fp32;
+ * the scores' gradient is rounded to the tensors' type once, relative to the largest row weight.  Loss, count,
+ * reductions and targets out of range as flb200_cce_forward; a row whose target is ignored or out of range
+ * adds nothing to any gradient.  Of the gradients any may be NULL; grad_w is of the weights' type or f32. */
+typedef struct flb200_linear_cce_desc {
+  int64_t rows, features, classes;
+  int32_t reduction;     /* FLB200_REDUCE_* */
+  int32_t ignore_index;
+  int32_t dtype;
+} flb200_linear_cce_desc;
+int flb200_linear_cce_supported(const flb200_linear_cce_desc* d);
+/* which: 0 forward, 1 backward; depends on the alignment of x and weight */
+size_t flb200_linear_cce_workspace_bytes(const flb200_linear_cce_desc* d, const void* x, const void* weight,
+                                         int which);
+int flb200_linear_cce_forward(const flb200_linear_cce_desc* d, const void* x, const void* weight,
+                              const float* bias, const int32_t* targets, float* loss, float* lse,
+                              int32_t* count_out, int32_t* bad_target_flag, void* workspace,
+                              size_t workspace_bytes, void* stream);
+int flb200_linear_cce_backward(const flb200_linear_cce_desc* d, const void* x, const void* weight,
+                               const float* bias, const float* lse, const float* grad_loss,
+                               const int32_t* targets, const int32_t* count, void* grad_x, void* grad_w,
+                               int grad_w_dtype, float* grad_bias, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
 /* ----------------------------------------------------------- rnn (a7, a8) */
 /* x [I,B,T], y [H*dirs,B,T], hx/cx/hy/cy [H,B,L*dirs]; w flat in the cuDNN
  * order the reference uses (flashlight/fl/nn/Utils.cpp:45-84;
