@@ -74,6 +74,15 @@ class LinearCceDesc(C.Structure):
                 ("dtype", i32)]
 
 
+class AttentionDesc(C.Structure):
+    _fields_ = [(n, i64) for n in ("batch", "q_len", "k_len", "heads", "kv_heads", "head_dim")] + [
+        ("scale", f32), ("softcap", f32), ("dtype", i32)]
+
+
+class HeadTensor(C.Structure):
+    _fields_ = [("data", vp), ("batch", i64), ("row", i64), ("head", i64)]
+
+
 P = C.POINTER
 # name -> (restype, argtypes); one entry per declaration in include/flb200.h
 SIGNATURES = {
@@ -154,6 +163,14 @@ SIGNATURES = {
     "flb200_attention_backward_workspace_bytes": (sz, [i64, i64, i64]),
     "flb200_attention_backward": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, f32,
                                             C.c_int, C.c_int, vp, sz, vp]),
+    "flb200_attention_mask_bytes": (sz, [i64, i64, i64]),
+    "flb200_attention_mask": (C.c_int, [i64, i64, i64, C.c_int, vp, vp, vp, vp]),
+    "flb200_masked_attention_supported": (C.c_int, [P(AttentionDesc)]),
+    "flb200_masked_attention_forward": (C.c_int, [P(AttentionDesc), P(HeadTensor), P(HeadTensor), P(HeadTensor),
+                                                  vp, vp, P(HeadTensor), vp, vp]),
+    "flb200_masked_attention_backward_workspace_bytes": (sz, [P(AttentionDesc)]),
+    "flb200_masked_attention_backward": (C.c_int, [P(AttentionDesc)] + [P(HeadTensor)] * 5 + [vp, vp, vp] +
+                                         [P(HeadTensor)] * 3 + [vp, sz, vp]),
     "flb200_sgd_step": (C.c_int, [vp, vp, vp, i64, f32, f32, f32, C.c_int, f32, C.c_int, C.c_int, vp]),
     "flb200_adamw_step": (C.c_int, [P(AdamwDesc), P(AdamwTensor), i64, vp]),
     "flb200_relu_forward_mask": (C.c_int, [vp, vp, vp, i64, C.c_int, vp]),

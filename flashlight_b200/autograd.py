@@ -734,6 +734,48 @@ def attention_packed(qkv: Variable, B: int, T: int, heads: int, scale: float,
     return Variable(out, False, [qkv], grad_func)
 
 
+def masked_attention(q: Variable, k: Variable, v: Variable, mask: F.AttentionMask, scale: float,
+                     softcap: float = 0.0, slopes: Optional[torch.Tensor] = None) -> Variable:
+    """softmax(softcap * tanh(scale q k^T / softcap) - slopes |i - j|) v where each query sees an interval of the
+    keys (functions.attention_mask: causal, documents of a packed row, a prefix): q (batch, length, heads, head
+    dim), k and v with as many heads or a divisor of them.  One kernel forward, which keeps the rows' log-sum-exp,
+    and one for the three gradients behind a small pass over the output's.  slopes take no gradient."""
+    qt, kt, vt = q.tensor, k.tensor, v.tensor
+    out, lse = F.masked_attention(qt, kt, vt, mask, scale, softcap, slopes)
+
+    def grad_func(inputs, gy):
+        grads = F.masked_attention_backward(qt, kt, vt, out, gy, lse, mask, scale, softcap, slopes)
+        for inp, g in zip(inputs, grads):
+            inp.addGrad(g)
+
+    return Variable(out, False, [q, k, v], grad_func)
+
+
+def masked_attention_packed(qkv: Variable, heads: int, mask: F.AttentionMask, scale: float, softcap: float = 0.0,
+                            slopes: Optional[torch.Tensor] = None, kv_heads: Optional[int] = None) -> Variable:
+    """masked_attention on the packed projection (batch * length, (heads + 2 key heads) * head dim), result (batch *
+    length, heads * head dim): q, k and v are read, and their gradients written, where they lie."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    t = qkv.tensor.contiguous()
+    B, T = mask.batch, mask.q_len
+    if t.shape[0] != B * T or mask.k_len != T or t.shape[1] % (heads + 2 * kv_heads):
+        raise ValueError("masked_attention_packed: qkv does not match the mask and the heads")
+    hd = t.shape[1] // (heads + 2 * kv_heads)
+
+    def parts(x):
+        x = x.view(B, T, heads + 2 * kv_heads, hd)
+        return x[:, :, :heads], x[:, :, heads:heads + kv_heads], x[:, :, heads + kv_heads:]
+
+    out, lse = F.masked_attention(*parts(t), mask, scale, softcap, slopes)
+
+    def grad_func(inputs, gy):
+        g = torch.empty_like(t)
+        F.masked_attention_backward(*parts(t), out, gy.reshape(out.shape), lse, mask, scale, softcap, slopes, parts(g))
+        inputs[0].addGrad(g)
+
+    return Variable(out.view(B * T, heads * hd), False, [qkv], grad_func)
+
+
 def softmax_rows(x: Variable, scale: float = 1.0, causal_period: int = 0) -> Variable:
     """softmax over the last dimension (Functions.cpp:1021-1042) of scale * x, with the causal
     mask of attention scores folded in when causal_period = T (x is a stack of T-row score

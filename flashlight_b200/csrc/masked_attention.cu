@@ -1,0 +1,1135 @@
+// Attention over the interval of keys that each query sees, with capped scores and a distance bias, forward and
+// gradient; f16 or bf16, head dimensions up to 128, key heads shared by several query heads:
+//     u = scale q.k / cap    z = cap tanh(u)  (cap 0: scale q.k)    s = z - slope_h |i - j|
+//     P = exp(s - lse) over j in [lo_i, hi_i), 0 elsewhere          o = P v
+//     dP = do v^T    D = rowsum(do o)    dS = P (dP - D) (1 - tanh(u)^2)
+//     dq = scale dS k    dk = scale dS^T q    dv = P^T do           (dk, dv summed over the heads that share them)
+// flashlight/fl/autograd/Functions.cpp:1828-1891 is the chain of whole-tensor operators for this, its mask an
+// additive tensor.  One interval per query says all that a causal mask, documents packed into a row, a prefix and
+// padding say together; flb200_attention_mask makes it once per batch, with what the kernels below need to know
+// of blocks of 128: which key blocks a query block meets, and whether all of a block is seen.
+//
+// The scores of a 128 x 128 block live in tensor memory only.  tanh(u) = 1 - 2 r, r = 1 / (1 + e^2u), from the
+// approximate exponential and reciprocal: its absolute error is below 2^-21 (the approximate tanh is 2^-11 off, at a
+// cap of 50 an error of 2 % in P), and 1 - tanh(u)^2 = 4 r (1 - r) comes with it.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <mutex>
+#include <set>
+#include <utility>
+
+#include "common.cuh"
+#include "flb200.h"
+#include "tc_core.cuh"
+#include "tc_gemm.cuh"
+
+namespace flb200 {
+namespace {
+
+using namespace tc;
+
+constexpr int kBlock = 128;        // queries and keys of a block
+constexpr int kBox = 128 * 128;    // bytes of [128 rows][64 16-bit values], one TMA box
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kThreads2 = 320;     // warps 0..7: two threads per row or a tile each; 8: TMA; 9: MMA
+
+// ------------------------------------------------------------------------------------------ the mask
+// rows: [lo, hi) of each query ([batch][q_len]; hi <= lo: it sees nothing).  q_blocks: of each block of queries the
+// least lo and the greatest hi of those that see something, and the greatest lo and the least hi of all (an
+// empty row makes that pair empty).  k_blocks: the query blocks [first, last) that may see a block of keys.
+struct MaskView {
+  const int2* rows;
+  const int4* q_blocks;
+  const int2* k_blocks;
+};
+__host__ __device__ inline int blocks_of(long long n) { return (int)((n + kBlock - 1) / kBlock); }
+inline size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
+size_t mask_bytes(long long batch, long long q_len, long long k_len) {
+  return round16(batch * blocks_of(q_len) * sizeof(int4)) + round16(batch * blocks_of(k_len) * sizeof(int2)) +
+         batch * q_len * sizeof(int2);
+}
+MaskView mask_view(const void* mask, long long batch, long long q_len, long long k_len) {
+  const char* p = static_cast<const char*>(mask);
+  MaskView v;
+  v.q_blocks = reinterpret_cast<const int4*>(p);
+  p += round16(batch * blocks_of(q_len) * sizeof(int4));
+  v.k_blocks = reinterpret_cast<const int2*>(p);
+  p += round16(batch * blocks_of(k_len) * sizeof(int2));
+  v.rows = reinterpret_cast<const int2*>(p);
+  return v;
+}
+
+// Inclusive running maximum over the CTA's 1024 threads, in thread order, of a carry and each thread's value.
+__device__ __forceinline__ int running_max(int v, int carry, int* scratch, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v = max(v, u);
+  }
+  __syncthreads();  // scratch may still be read from the call before
+  if (lane == 31) scratch[warp] = v;
+  __syncthreads();
+  int before = carry;
+  for (int w = 0; w < warp; ++w) before = max(before, scratch[w]);
+  *total = carry;
+  for (int w = 0; w < 32; ++w) *total = max(*total, scratch[w]);
+  return max(v, before);
+}
+
+// One CTA per row of the batch: a query's document is the run of equal ids around its position, and the ends of the
+// runs are a running maximum from the left and one from the right.
+constexpr int kRun = 4;  // positions of a thread
+__global__ void __launch_bounds__(1024)
+attention_mask_kernel(const int* __restrict__ documents, const int* __restrict__ prefix, int q_len, int k_len,
+                      int causal, int4* __restrict__ q_blocks, int2* __restrict__ k_blocks, int2* __restrict__ rows) {
+  chain_begin();
+  __shared__ int scratch[32];
+  const int b = blockIdx.x, off = k_len - q_len, step = 1024 * kRun;
+  const int nq = blocks_of(q_len), nk = blocks_of(k_len);
+  const int* ids = documents ? documents + (long long)b * k_len : nullptr;
+  const int seen_by_all = prefix ? min(max(prefix[b], 0), k_len) : 0;
+  rows += (long long)b * q_len;
+  q_blocks += (long long)b * nq;
+  k_blocks += (long long)b * nk;
+  if (!ids) {
+    for (int i = threadIdx.x; i < q_len; i += 1024)
+      rows[i] = make_int2(0, causal ? max(i + off + 1, seen_by_all) : k_len);
+  } else {
+    int carry = 0;
+    for (int p0 = 0; p0 < k_len; p0 += step) {
+      int start[kRun], id[kRun], last = 0;
+      const int p = p0 + threadIdx.x * kRun;
+      int before = p > 0 && p < k_len ? ids[p - 1] : 0;
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        id[j] = p + j < k_len ? ids[p + j] : 0;
+        if (p + j < k_len && (p + j == 0 || id[j] != before)) last = p + j;
+        start[j] = last;
+        before = id[j];
+      }
+      int total;
+      // (of the threads before; this one's own runs come on top)
+      const int through = running_max(last, carry, scratch, &total);
+      const int mine = __shfl_up_sync(0xffffffffu, through, 1);
+      int left = carry;
+      if ((threadIdx.x & 31) > 0) left = mine;
+      else for (int w = 0; w < (int)(threadIdx.x >> 5); ++w) left = max(left, scratch[w]);
+      carry = total;
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        const int i = p + j - off;
+        if (p + j < k_len && i >= 0)
+          rows[i] = id[j] < 0 ? make_int2(0, 0)
+                              : make_int2(max(start[j], left), causal ? p + j + 1 : k_len);
+      }
+    }
+    if (!causal || seen_by_all > 0) {  // the runs' ends count
+      int from_right = 0;  // k_len - end, running
+      const int last0 = (k_len - 1) / step * step;
+      for (int p0 = last0; p0 >= 0; p0 -= step) {
+        // thread t looks at positions from the right: the chunk's last kRun positions are thread 0's
+        const int p = p0 + step - 1 - threadIdx.x * kRun;
+        int end[kRun], id[kRun], last = 0;
+        int behind = p + 1 < k_len ? ids[p + 1] : 0;
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+          id[j] = p - j < k_len ? ids[p - j] : 0;
+          if (p - j < k_len && p - j + 1 < k_len && id[j] != behind) last = k_len - (p - j + 1);
+          end[j] = last;
+          behind = id[j];
+        }
+        int total;
+        const int through = running_max(last, from_right, scratch, &total);
+        const int mine = __shfl_up_sync(0xffffffffu, through, 1);
+        int right = from_right;
+        if ((threadIdx.x & 31) > 0) right = mine;
+        else for (int w = 0; w < (int)(threadIdx.x >> 5); ++w) right = max(right, scratch[w]);
+        from_right = total;
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+          const int i = p - j - off;
+          if (p - j < k_len && i >= 0 && id[j] >= 0) {
+            const int e = k_len - max(end[j], right);
+            rows[i].y = causal ? min(e, max(p - j + 1, seen_by_all)) : e;
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  for (int i = threadIdx.x >> 5; i < nq; i += 32) {
+    int lo_min = 0x7fffffff, hi_max = 0, lo_max = 0, hi_min = 0x7fffffff;
+    for (int r = i * kBlock + lane; r < min(q_len, (i + 1) * kBlock); r += 32) {
+      const int2 x = rows[r];
+      if (x.y > x.x) {
+        lo_min = min(lo_min, x.x);
+        hi_max = max(hi_max, x.y);
+        lo_max = max(lo_max, x.x);
+        hi_min = min(hi_min, x.y);
+      } else {
+        lo_max = 0x7fffffff;
+        hi_min = 0;
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      lo_min = min(lo_min, __shfl_xor_sync(0xffffffffu, lo_min, o));
+      hi_max = max(hi_max, __shfl_xor_sync(0xffffffffu, hi_max, o));
+      lo_max = max(lo_max, __shfl_xor_sync(0xffffffffu, lo_max, o));
+      hi_min = min(hi_min, __shfl_xor_sync(0xffffffffu, hi_min, o));
+    }
+    if (lane == 0) q_blocks[i] = make_int4(lo_min, hi_max, lo_max, hi_min);
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j < nk; j += 1024) {
+    int first = nq, last = 0;
+    for (int i = 0; i < nq; ++i) {
+      const int4 q = q_blocks[i];
+      if (q.x < (j + 1) * kBlock && q.y > j * kBlock) {
+        first = min(first, i);
+        last = i + 1;
+      }
+    }
+    k_blocks[j] = make_int2(first, last);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ common parts
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+#define FLB200_R32(r)                                                                                       \
+  "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),           \
+      "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), \
+      "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),            \
+      "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),            \
+      "+r"(r[30]), "+r"(r[31])
+// 32 columns of this thread's lane; the registers may be used after wait_ld and settle only
+__device__ __forceinline__ void ld32_begin(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void settle(uint32_t* r) { asm volatile("" : FLB200_R32(r)); }
+__device__ __forceinline__ void st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D[tmem] += A[tmem] B[smem]: a row of A per lane, two 16-bit k per column
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// A tile of 128 rows and D columns is D / 64 boxes.  As a K-major operand (a row per m or n) k advances 32 bytes per 16
+// inside a box, rows 128 bytes; as an MN-major one (a row per k) k advances 2048 bytes per 16.
+template <int D>
+__device__ __forceinline__ uint64_t k_major(const char* tile) { return umma_desc(smem_u32(tile), 16, 1024, 2); }
+template <int D>
+__device__ __forceinline__ uint64_t mn_major(const char* tile) { return umma_desc(smem_u32(tile), kBox, 1024, 2); }
+__device__ __forceinline__ uint32_t k_step(int kk) { return (uint32_t)((kk >> 2) * kBox + (kk & 3) * 32); }
+
+template <int D>
+__device__ __forceinline__ void load_tile(const CUtensorMap* map, uint64_t* bar, char* to, int row0, int head,
+                                          int batch) {
+#pragma unroll
+  for (int x = 0; x < D; x += 64) {
+    int c[4] = {x, row0, head, batch};
+    tma_load(map, bar, to + x / 64 * kBox, 4, c);
+  }
+}
+
+struct OutTensor {  // element (batch b, row t, head h, d) at b * batch + t * row + h * head + d
+  void* p;
+  long long batch, row, head;
+};
+// 32 columns from c0 on of a row, of which those in front of head_dim exist
+template <typename T>
+__device__ __forceinline__ void store_row(const OutTensor& o, int b, int t, int h, int c0, int head_dim,
+                                          const uint32_t* v, float factor) {
+  T* to = static_cast<T*>(o.p) + b * o.batch + t * o.row + h * o.head + c0;
+  const auto two = [&](int e) {
+    return pack2<T>(__uint_as_float(v[e]) * factor, __uint_as_float(v[e + 1]) * factor);
+  };
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (c0 + 8 * u < head_dim)
+      *reinterpret_cast<uint4*>(to + 8 * u) = make_uint4(two(8 * u), two(8 * u + 2), two(8 * u + 4), two(8 * u + 6));
+}
+
+struct AttnShape {
+  int q_len, k_len, heads, group, head_dim;  // group: query heads per key head
+  MaskView mask;
+  const float* slopes;
+  float to_log2;     // scale * log2 e (no cap)
+  float cap_log2;    // cap * log2 e
+  float to_2u_log2;  // 2 scale / cap * log2 e
+  float scale;
+  int* status;
+};
+
+// ------------------------------------------------------------------------------------------ forward
+// One CTA takes 256 queries of a head, as two tiles with four warps each (a thread per row); the tiles
+// share the keys' blocks, and while one tile's warps are at its softmax the tensor pipe is at the other's products:
+//     S_t = Q_t K_j^T    columns 128 t ..         P_t over the same columns, 16 bits, the A operand of
+//     O_t += P_t V_j     columns 256 + D t ..     (kept over j)
+// P is exp2 of the scores less a reference that is raised, and O rescaled, only where a row's maximum passed
+// it by more than 2^8: rarely behind the first blocks.  P up to 2^8 loses nothing in either type.
+template <int D>
+struct FwdSmem {
+  static constexpr int kTile = D / 64 * kBox, kStages = D == 64 ? 3 : 2;
+  static constexpr int kTotal = 2 * kTile + 2 * kStages * kTile + 1024 + 256;
+};
+struct AttnFwdArgs {
+  AttnShape s;
+  OutTensor out;
+  float* lse;  // [batch][heads][q_len], or null
+  int pairs;
+};
+
+template <int D, typename T, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreads2, 1)
+masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v, const AttnFwdArgs a) {
+  chain_begin();
+  using SM = FwdSmem<D>;
+  constexpr int kStages = SM::kStages, kTile = SM::kTile;
+  extern __shared__ __align__(1024) char smem_raw[];
+  char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  char *sQ = base, *sK = base + 2 * kTile, *sV = sK + kStages * kTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + kStages * kTile);
+  uint64_t *bar_q = bars, *k_full = bars + 1, *k_empty = k_full + kStages, *v_full = k_empty + kStages,
+           *v_empty = v_full + kStages, *bar_s = v_empty + kStages, *bar_p = bar_s + 2, *bar_o = bar_p + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_o + 2);
+  volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int pair = a.pairs - 1 - (int)blockIdx.x % a.pairs;  // the longest of a causal head first
+  const int bh = blockIdx.x / a.pairs, batch = bh / a.s.heads, head = bh - batch * a.s.heads;
+  const int nq = blocks_of(a.s.q_len), off = a.s.k_len - a.s.q_len;
+
+  // the key blocks of the two tiles
+  int begin[2], end[2];
+  int4 info[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    info[t] = make_int4(0, 0, 0, 0);
+    if (2 * pair + t < nq) info[t] = a.s.mask.q_blocks[(long long)batch * nq + 2 * pair + t];
+    begin[t] = end[t] = 0;
+    if (info[t].y > info[t].x) {
+      begin[t] = info[t].x / kBlock;
+      end[t] = blocks_of(info[t].y);
+    }
+  }
+  const bool both = end[0] > begin[0] && end[1] > begin[1];
+  const int j0 = both ? min(begin[0], begin[1]) : (end[0] > begin[0] ? begin[0] : begin[1]);
+  const int j1 = max(end[0], end[1]);  // (j1 = j0 = 0 where neither sees anything)
+
+  if (threadIdx.x == 0) {
+    mbar_init(bar_q, 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&bar_s[t], 1);
+      mbar_init(&bar_p[t], 4);
+      mbar_init(&bar_o[t], 1);
+    }
+    *failed = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
+    if (*failed == 0 && !mbar_wait(bar, phase)) *failed = code;
+    tc_fence_after();
+  };
+
+  if (warp == 8) {
+    if (j1 > j0 && elect_one()) {
+      const int tiles = 2 * pair + 1 < nq ? 2 : 1;
+      mbar_expect_tx(bar_q, tiles * kTile);
+      for (int t = 0; t < tiles; ++t)
+        load_tile<D>(&map_q, bar_q, sQ + t * kTile, (2 * pair + t) * kBlock, head, batch);
+      const int kv = head / a.s.group;
+      uint32_t s = 0, round = 0;
+      for (int j = j0; j < j1; ++j) {
+        if (round > 0) wait(&k_empty[s], (round - 1) & 1, 1);
+        mbar_expect_tx(&k_full[s], kTile);
+        load_tile<D>(&map_k, &k_full[s], sK + s * kTile, j * kBlock, kv, batch);
+        if (round > 0) wait(&v_empty[s], (round - 1) & 1, 2);
+        mbar_expect_tx(&v_full[s], kTile);
+        load_tile<D>(&map_v, &v_full[s], sV + s * kTile, j * kBlock, kv, batch);
+        if (++s == kStages) { s = 0; ++round; }
+      }
+    }
+  } else if (warp == 9) {
+    if (j1 > j0 && elect_one()) {
+      constexpr int kOperand = std::is_same<T, __half>::value ? kOperandF16 : kOperandBf16;
+      const uint32_t id_s = umma_idesc_f16(kOperand, kBlock, 0, 0), id_o = umma_idesc_f16(kOperand, D, 0, 1);
+      const uint64_t dQ = k_major<D>(sQ), dK = k_major<D>(sK), dV = mn_major<D>(sV);
+      auto active = [&](int t, int j) { return j >= begin[t] && j < end[t]; };
+      auto scores = [&](int t, uint32_t s) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_f16(tmem + 128 * t, umma_desc_advance(dQ, t * kTile + k_step(kk)),
+                   umma_desc_advance(dK, s * kTile + k_step(kk)), id_s, kk > 0);
+        umma_commit(&bar_s[t]);
+      };
+      uint32_t done[2] = {0, 0};  // blocks of each tile
+      uint32_t ks = 0, k_round = 0, vs = 0, v_round = 0;
+      wait(bar_q, 0, 3);
+      wait(&k_full[0], 0, 4);
+      for (int t = 0; t < 2; ++t)
+        if (active(t, j0)) scores(t, 0);
+      umma_commit(&k_empty[0]);
+      if (++ks == kStages) { ks = 0; ++k_round; }
+      for (int j = j0; j < j1; ++j) {
+        bool next_here = false;
+        for (int t = 0; t < 2; ++t) {
+          if (active(t, j)) {
+            wait(&bar_p[t], done[t] & 1, 5);
+            wait(&v_full[vs], v_round & 1, 6);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)  // K = 128 keys
+              umma_f16_ts(tmem + 256 + D * t, tmem + 128 * t + 8 * kk,
+                          umma_desc_advance(dV, vs * kTile + kk * 2048), id_o, (done[t] > 0 || kk > 0) ? 1u : 0u);
+            umma_commit(&bar_o[t]);
+            ++done[t];
+          }
+          if (j + 1 < j1 && active(t, j + 1)) {
+            if (!next_here) wait(&k_full[ks], k_round & 1, 7);
+            next_here = true;
+            scores(t, ks);
+          }
+        }
+        // (a block that neither tile meets is loaded all the same, and handed back)
+        if (!active(0, j) && !active(1, j)) wait(&v_full[vs], v_round & 1, 6);
+        umma_commit(&v_empty[vs]);
+        if (++vs == kStages) { vs = 0; ++v_round; }
+        if (j + 1 < j1) {
+          if (!next_here) wait(&k_full[ks], k_round & 1, 7);
+          umma_commit(&k_empty[ks]);
+          if (++ks == kStages) { ks = 0; ++k_round; }
+        }
+      }
+    }
+  } else {
+    const int t = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const int q = (2 * pair + t) * kBlock + row;
+    const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_addr = lane_addr + 128u * t, o_addr = lane_addr + 256u + (uint32_t)(D * t);
+    int2 seen = make_int2(0, 0);
+    if (q < a.s.q_len) seen = a.s.mask.rows[(long long)batch * a.s.q_len + q];
+    const float slope = BIAS ? a.s.slopes[head] * kLog2e : 0.f;
+    const float pos = (float)(q + off);
+    float ref = -1e30f, sum = 0.f;  // in powers of 2; a row that has seen nothing yet is far below all scores
+    const int blocks = end[t] - begin[t];
+    for (int it = 0; it < blocks; ++it) {
+      const int key0 = (begin[t] + it) * kBlock;
+      uint32_t raw[4][32];
+      wait(&bar_s[t], it & 1, 8);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) ld32_begin(s_addr + 32 * c, raw[c]);
+      wait_ld();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) settle(raw[c]);
+      float s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int e = 0; e < 32; ++e) s[c][e] = __uint_as_float(raw[c][e]);
+      // The scores in powers of 2.  (Without cap and bias they stay as they are, the factor is positive and comes
+      // with the subtraction below.)
+      if constexpr (CAP || BIAS) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            float z = CAP ? fmaf(-2.f * a.s.cap_log2, rcp(1.f + ex2(s[c][e] * a.s.to_2u_log2)), a.s.cap_log2)
+                          : s[c][e] * a.s.to_log2;
+            if (BIAS) z = fmaf(-slope, fabsf(pos - (float)(key0 + 32 * c + e)), z);
+            s[c][e] = z;
+          }
+      }
+      // (blocks that all rows see whole need no test per element)
+      if (!(info[t].z <= key0 && info[t].w >= key0 + kBlock)) {
+        const unsigned width = (unsigned)max(seen.y - seen.x, 0);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if ((unsigned)(key0 + 32 * c + e - seen.x) >= width) s[c][e] = -INFINITY;
+      }
+      float mx4[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mx4[c] = s[c][0];
+#pragma unroll
+        for (int e = 1; e < 32; ++e) mx4[c] = fmaxf(mx4[c], s[c][e]);
+      }
+      float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      if constexpr (!CAP && !BIAS) mx *= a.s.to_log2;
+      const bool raise = mx > ref + 8.f;
+      if (__any_sync(0xffffffffu, raise)) {
+        const float next = raise ? mx : ref, alpha = raise ? ex2(ref - next) : 1.f;
+        ref = next;
+        sum *= alpha;
+        if (it > 0) {
+          wait(&bar_o[t], (it - 1) & 1, 9);
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            ld32_begin(o_addr + c, o);
+            wait_ld();
+            settle(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            st32(o_addr + c, o);
+          }
+        }
+      }
+      float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; c += 2) {
+        uint32_t p[32];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float p0, p1;
+            if constexpr (CAP || BIAS) {
+              p0 = ex2(s[c + h][e] - ref);
+              p1 = ex2(s[c + h][e + 1] - ref);
+            } else {
+              p0 = ex2(fmaf(s[c + h][e], a.s.to_log2, -ref));
+              p1 = ex2(fmaf(s[c + h][e + 1], a.s.to_log2, -ref));
+            }
+            sum4[(e >> 1) & 3] += p0 + p1;
+            p[16 * h + e / 2] = pack2<T>(p0, p1);
+          }
+        st32(s_addr + 16 * c, p);
+      }
+      sum += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+      wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive(&bar_p[t]);
+    }
+    if (blocks > 0) wait(&bar_o[t], (blocks - 1) & 1, 10);
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll 1
+    for (int c = 0; c < D; c += 32) {
+      uint32_t o[32];
+      __syncwarp();  // the lanes past the end store nothing, and are back for the next load
+      if (blocks > 0) {
+        ld32_begin(o_addr + c, o);
+        wait_ld();
+        settle(o);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0;
+      }
+      if (q < a.s.q_len)
+        store_row<T>(a.out, batch, q, head, c, a.s.head_dim, o, inv);
+    }
+    // NaN among the scores shows in both
+    if (q < a.s.q_len && a.lse)
+      a.lse[(long long)bh * a.s.q_len + q] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
+  }
+  if (*failed)  // copies and contractions under way when a wait ran out have ended after this
+    for (const long long t0 = clock64(); clock64() - t0 < 100000;) {
+    }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *failed != 0 && a.s.status) atomicExch(a.s.status, *failed);
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ gradient
+// Two kinds of CTA in one launch, alike but for what their rows are.  A tile of 128 rows stays in shared memory, the
+// other side comes by in blocks of 128 columns, as two halves with four warps each (a thread per row):
+//     dK, dV   rows = keys K_j V_j     columns = queries Q_i dO_i of all heads that share the key head
+//     dQ       rows = queries Q_i dO_i columns = keys K_j V_j
+//     S = rows1 cols1^T, dP = rows2 cols2^T     (128 x 64 each, columns 128 half .. of tensor memory)
+//     P and dS over the same columns, 16 bits, A operands of
+//     dV += P cols2, dK += dS cols1   or   dQ += dS cols1     (columns 256 ..)
+// Nothing is added across CTAs: the result does not depend on their order.  The price is that S and dP are made
+// twice, 7 contractions where sums in device memory need 5; those would cost 4 bytes a value per key block.
+template <int D>
+struct BwdSmem {
+  static constexpr int kTile = D / 64 * kBox, kStages = 2;
+  static constexpr int kColumns = 2 * 128 * 16;  // two buffers of (lse, D, lo, hi) per query column
+  static constexpr int kTotal = 2 * kTile + 2 * kStages * kTile + kColumns + 1024 + 256;
+};
+struct AttnBwdArgs {
+  AttnShape s;
+  const float* lse;   // [batch][heads][q_len]
+  const float* dsum;  // the same of D
+  OutTensor dq, dk, dv;
+  int kv_ctas;        // the first of the grid: dK and dV
+};
+
+template <int D, typename T, bool CAP, bool BIAS, bool KV>
+__device__ __forceinline__ void
+backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, const CUtensorMap& map_do,
+              const AttnBwdArgs& a, int cta) {
+  using SM = BwdSmem<D>;
+  constexpr int kStages = SM::kStages, kTile = SM::kTile;
+  extern __shared__ __align__(1024) char smem_raw[];
+  char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  char *sR1 = base, *sR2 = base + kTile, *sC1 = base + 2 * kTile, *sC2 = sC1 + kStages * kTile;
+  float4* columns = reinterpret_cast<float4*>(sC2 + kStages * kTile);  // [2][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(columns + 256);
+  uint64_t *bar_r = bars, *full = bars + 1, *empty = full + kStages, *bar_s = empty + kStages, *bar_p = bar_s + 2,
+           *bar_a = bar_p + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_a + 1);
+  volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int nq = blocks_of(a.s.q_len), nk = blocks_of(a.s.k_len), off = a.s.k_len - a.s.q_len;
+  const int per_head = KV ? nk : nq, heads = KV ? a.s.heads / a.s.group : a.s.heads;
+  const int block = KV ? cta % per_head : per_head - 1 - cta % per_head;  // (the longest of a causal head first)
+  const int bh = cta / per_head, batch = bh / heads, head = bh - batch * heads;
+  int first, count, total;  // column blocks, and how many there are over all heads
+  int4 info = make_int4(0, 0, 0, 0);
+  if (KV) {
+    const int2 r = a.s.mask.k_blocks[(long long)batch * nk + block];
+    first = r.x;
+    count = max(r.y - r.x, 0);
+    total = count * a.s.group;
+  } else {
+    info = a.s.mask.q_blocks[(long long)batch * nq + block];
+    first = info.y > info.x ? info.x / kBlock : 0;
+    count = info.y > info.x ? blocks_of(info.y) - first : 0;
+    total = count;
+  }
+
+  if (threadIdx.x == 0) {
+    mbar_init(bar_r, 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(&bar_s[h], 1);
+      mbar_init(&bar_p[h], 4);
+    }
+    mbar_init(bar_a, 1);
+    *failed = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
+    if (*failed == 0 && !mbar_wait(bar, phase)) *failed = code;
+    tc_fence_after();
+  };
+
+  if (warp == 8) {
+    if (total > 0 && elect_one()) {
+      mbar_expect_tx(bar_r, 2 * kTile);
+      load_tile<D>(KV ? &map_k : &map_q, bar_r, sR1, block * kBlock, head, batch);
+      load_tile<D>(KV ? &map_v : &map_do, bar_r, sR2, block * kBlock, head, batch);
+      uint32_t s = 0, round = 0;
+      int in_head = 0, h = KV ? head * a.s.group : head / a.s.group;
+      for (int it = 0; it < total; ++it) {
+        if (round > 0) wait(&empty[s], (round - 1) & 1, 1);
+        mbar_expect_tx(&full[s], 2 * kTile);
+        load_tile<D>(KV ? &map_q : &map_k, &full[s], sC1 + s * kTile, (first + in_head) * kBlock, h, batch);
+        load_tile<D>(KV ? &map_do : &map_v, &full[s], sC2 + s * kTile, (first + in_head) * kBlock, h, batch);
+        if (++s == kStages) { s = 0; ++round; }
+        if (++in_head == count) { in_head = 0; ++h; }
+      }
+    }
+  } else if (warp == 9) {
+    if (total > 0 && elect_one()) {
+      constexpr int kOperand = std::is_same<T, __half>::value ? kOperandF16 : kOperandBf16;
+      const uint32_t id_s = umma_idesc_f16(kOperand, 64, 0, 0), id_a = umma_idesc_f16(kOperand, D, 0, 1);
+      const uint64_t dR1 = k_major<D>(sR1), dR2 = k_major<D>(sR2), dC1 = k_major<D>(sC1), dC2 = k_major<D>(sC2);
+      const uint64_t mC1 = mn_major<D>(sC1), mC2 = mn_major<D>(sC2);
+      auto scores = [&](int h, uint32_t s) {  // rows 64 h .. of the column tiles
+        const uint32_t at = s * kTile + h * 8192;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_f16(tmem + 128 * h, umma_desc_advance(dR1, k_step(kk)), umma_desc_advance(dC1, at + k_step(kk)), id_s,
+                   kk > 0);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_f16(tmem + 128 * h + 64, umma_desc_advance(dR2, k_step(kk)), umma_desc_advance(dC2, at + k_step(kk)),
+                   id_s, kk > 0);
+        umma_commit(&bar_s[h]);
+      };
+      uint32_t s = 0, round = 0;
+      wait(bar_r, 0, 2);
+      wait(&full[0], 0, 3);
+      scores(0, 0);
+      scores(1, 0);
+      for (int it = 0; it < total; ++it) {
+        const uint32_t ns = s + 1 == kStages ? 0 : s + 1, nround = s + 1 == kStages ? round + 1 : round;
+        for (int h = 0; h < 2; ++h) {
+          wait(&bar_p[h], it & 1, 4);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {  // K = 64 columns of this half
+            const uint32_t at = s * kTile + h * 8192 + kk * 2048, add = (it > 0 || h > 0 || kk > 0) ? 1u : 0u;
+            if (KV)
+              umma_f16_ts(tmem + 256, tmem + 128 * h + 8 * kk, umma_desc_advance(mC2, at), id_a, add);
+            umma_f16_ts(tmem + 256 + (KV ? D : 0), tmem + 128 * h + 64 + 8 * kk, umma_desc_advance(mC1, at), id_a, add);
+          }
+          if (h == 1) umma_commit(it + 1 < total ? &empty[s] : bar_a);
+          if (it + 1 < total) {
+            if (h == 0) wait(&full[ns], nround & 1, 3);
+            scores(h, ns);
+          }
+        }
+        s = ns;
+        round = nround;
+      }
+    }
+  } else {
+    const int h = warp >> 2;                    // which half of the columns
+    const int row = (warp & 3) * 32 + lane;
+    const int mine = block * kBlock + row;      // key or query
+    const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_addr = lane_addr + 128u * h;
+    const int tid = threadIdx.x & 127;          // in the half's four warps
+    const long long rows0 = (long long)(KV ? batch * a.s.heads + head * a.s.group : bh) * a.s.q_len;
+    // (a row that sees nothing, and what lies past the end: lse of infinity makes P zero)
+    auto lse_of = [&](long long at) {
+      const float l = a.lse[at];
+      return l == -INFINITY ? INFINITY : l * kLog2e;
+    };
+    float my_lse = INFINITY, my_d = 0.f, slope = 0.f;
+    int2 seen = make_int2(0, 0);
+    if (!KV && mine < a.s.q_len) {
+      my_lse = lse_of(rows0 + mine);
+      my_d = a.dsum[rows0 + mine];
+      seen = a.s.mask.rows[(long long)batch * a.s.q_len + mine];
+    }
+    if (BIAS && !KV) slope = a.s.slopes[head] * kLog2e;
+    // of a query block's columns: lse, D and the interval, a thread per column
+    auto column = [&](int in_head, int hq) {
+      float4 c = make_float4(INFINITY, 0.f, 0.f, 0.f);
+      const int q = (first + in_head) * kBlock + 64 * h + tid;
+      if (tid < 64 && q < a.s.q_len) {
+        const int2 r = a.s.mask.rows[(long long)batch * a.s.q_len + q];
+        c = make_float4(lse_of(rows0 + (long long)hq * a.s.q_len + q), a.dsum[rows0 + (long long)hq * a.s.q_len + q],
+                        __int_as_float(r.x), __int_as_float(r.y));
+      }
+      return c;
+    };
+    if (KV && total > 0 && tid < 64) columns[64 * h + tid] = column(0, 0);
+    int in_head = 0, hq = 0;
+    for (int it = 0; it < total; ++it) {
+      const int col0 = (first + in_head) * kBlock + 64 * h;  // first column of this half
+      const float4* cols = columns + (it & 1) * 128 + 64 * h;
+      bool whole;
+      float4 ahead;
+      int next_in = in_head + 1, next_hq = hq;
+      if (next_in == count) { next_in = 0; ++next_hq; }
+      if (KV) {
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + h) : "memory");  // the columns are there
+        const int4 q = a.s.mask.q_blocks[(long long)batch * nq + first + in_head];
+        whole = q.z <= block * kBlock && q.w >= (block + 1) * kBlock;
+        if (BIAS) slope = a.s.slopes[head * a.s.group + hq] * kLog2e;
+        if (it + 1 < total) ahead = column(next_in, next_hq);
+      } else {
+        whole = info.z <= col0 && info.w >= col0 + 64;
+      }
+      wait(&bar_s[h], it & 1, 5);
+      const float apart = (float)(KV ? mine - col0 - off : mine + off - col0);  // of this row and column col0
+      // 32 columns at a time: P and dS lie over columns that have been read
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t sr[32], dr[32];
+        ld32_begin(s_addr + 32 * c, sr);
+        ld32_begin(s_addr + 64 + 32 * c, dr);
+        wait_ld();
+        settle(sr);
+        settle(dr);
+        uint32_t p[16], ds[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          float p2[2], ds2[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int col = 32 * c + e + k;
+            float4 x;
+            if (KV) x = cols[col];
+            float lse = KV ? x.x : my_lse, z = __uint_as_float(sr[e + k]), flat = 1.f;
+            if (BIAS) lse = fmaf(slope, fabsf(apart - (float)col), lse);
+            if (CAP) {
+              const float r = rcp(1.f + ex2(z * a.s.to_2u_log2));
+              z = fmaf(-2.f * a.s.cap_log2, r, a.s.cap_log2) - lse;
+              flat = 4.f * fmaf(-r, r, r);
+            } else {
+              z = fmaf(z, a.s.to_log2, -lse);
+            }
+            p2[k] = ex2(z);
+            ds2[k] = p2[k] * (__uint_as_float(dr[e + k]) - (KV ? x.y : my_d));
+            if (CAP) ds2[k] *= flat;
+            if (!whole) {  // what is not seen counts nothing, whatever its score
+              const bool sees = KV ? mine >= __float_as_int(x.z) && mine < __float_as_int(x.w)
+                                   : col0 + col >= seen.x && col0 + col < seen.y;
+              if (!sees) p2[k] = ds2[k] = 0.f;
+            }
+          }
+          p[e / 2] = pack2<T>(p2[0], p2[1]);
+          ds[e / 2] = pack2<T>(ds2[0], ds2[1]);
+        }
+        if (KV) st16(s_addr + 16 * c, p);
+        st16(s_addr + 64 + 16 * c, ds);
+      }
+      wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive(&bar_p[h]);
+      // (the other buffer was last read before this block's barrier)
+      if (KV && it + 1 < total && tid < 64) columns[((it + 1) & 1) * 128 + 64 * h + tid] = ahead;
+      in_head = next_in;
+      hq = next_hq;
+    }
+    if (total > 0) wait(bar_a, 0, 6);
+    // dV and dK: one per half of the warps; dQ: half of the columns each
+    const int c_first = KV ? 0 : h * (D / 2), c_last = KV ? D : c_first + D / 2;
+    const uint32_t from = lane_addr + 256u + (uint32_t)(KV ? D * h : 0);
+    const OutTensor out = KV ? (h == 0 ? a.dv : a.dk) : a.dq;
+    const float factor = KV && h == 0 ? 1.f : a.s.scale;
+    const int rows = KV ? a.s.k_len : a.s.q_len;
+#pragma unroll 1
+    for (int c = c_first; c < c_last; c += 32) {
+      uint32_t o[32];
+      __syncwarp();
+      if (total > 0) {
+        ld32_begin(from + c, o);
+        wait_ld();
+        settle(o);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0;
+      }
+      if (mine < rows)
+        store_row<T>(out, batch, mine, head, c, a.s.head_dim, o, factor);
+    }
+  }
+  if (*failed)
+    for (const long long t0 = clock64(); clock64() - t0 < 100000;) {
+    }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *failed != 0 && a.s.status) atomicExch(a.s.status, *failed);
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int D, typename T, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreads2, 1)
+masked_backward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                       const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
+                       const AttnBwdArgs a) {
+  chain_begin();
+  if ((int)blockIdx.x < a.kv_ctas)
+    backward_body<D, T, CAP, BIAS, true>(map_q, map_k, map_v, map_do, a, blockIdx.x);
+  else
+    backward_body<D, T, CAP, BIAS, false>(map_q, map_k, map_v, map_do, a, blockIdx.x - a.kv_ctas);
+}
+
+// D = rowsum(dO * O): sixteen lanes per row, one 16-byte load each.  Results in [batch][heads][q_len].
+template <typename T>
+__global__ void __launch_bounds__(256)
+masked_dsum_kernel(const OutTensor o, const OutTensor go, float* __restrict__ dsum, long long rows, int q_len,
+                   int heads, int head_dim) {
+  chain_begin();
+  const long long t = blockIdx.x * 256LL + threadIdx.x, r = t >> 4;
+  const int c = 8 * (int)(t & 15);
+  float acc = 0.f;
+  long long bt = 0, b = 0;
+  int h = 0;
+  if (r < rows) {
+    bt = r / heads;
+    h = (int)(r - bt * heads);
+    b = bt / q_len;
+    if (c < head_dim) {
+      const long long i = bt - b * q_len;
+      float x[8], g[8];
+      unpack16(load16(static_cast<const T*>(o.p) + b * o.batch + i * o.row + h * o.head + c), x);
+      unpack16(load16(static_cast<const T*>(go.p) + b * go.batch + i * go.row + h * go.head + c), g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc = fmaf(x[e], g[e], acc);
+    }
+  }
+#pragma unroll
+  for (int k = 1; k < 16; k <<= 1) acc += __shfl_xor_sync(0xffffffffu, acc, k);
+  if (r < rows && c == 0) dsum[(b * heads + h) * q_len + bt - b * q_len] = acc;
+}
+
+// ------------------------------------------------------------------------------------------ host
+int head_map(CUtensorMap* m, const flb200_head_tensor& t, long long batch, long long heads, long long len,
+             long long head_dim, int operand) {
+  const uint64_t dims[4] = {(uint64_t)head_dim, (uint64_t)len, (uint64_t)heads, (uint64_t)batch};
+  const uint64_t strides[3] = {(uint64_t)t.row * 2, (uint64_t)t.head * 2, (uint64_t)t.batch * 2};
+  const uint32_t box[4] = {64, kBlock, 1, 1};
+  return make_tensor_map(m, t.data, 4, dims, strides, box, kMapKMajor, nullptr, operand);
+}
+int configure(const void* kernel, int smem) {
+  static std::mutex mu;
+  static std::set<std::pair<int, const void*>> done;
+  int dev = 0;
+  FLB200_CUDA_CHECK(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count({dev, kernel})) return FLB200_OK;
+  FLB200_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  done.insert({dev, kernel});
+  return FLB200_OK;
+}
+OutTensor out_of(const flb200_head_tensor& t) { return OutTensor{t.data, t.batch, t.row, t.head}; }
+
+AttnShape shape_of(const flb200_attention_desc* d, const float* slopes, const void* mask) {
+  AttnShape s{};
+  s.q_len = (int)d->q_len;
+  s.k_len = (int)d->k_len;
+  s.heads = (int)d->heads;
+  s.group = (int)(d->heads / d->kv_heads);
+  s.head_dim = (int)d->head_dim;
+  s.mask = mask_view(mask, d->batch, d->q_len, d->k_len);
+  s.slopes = slopes;
+  s.scale = d->scale;
+  s.to_log2 = d->scale * kLog2e;
+  s.cap_log2 = d->softcap * kLog2e;
+  s.to_2u_log2 = d->softcap > 0.f ? 2.f * d->scale / d->softcap * kLog2e : 0.f;
+  s.status = status_ptr();
+  return s;
+}
+int check_attention(const char* name, const flb200_attention_desc* d) {
+  FLB200_REQUIRE(d, "%s: null descriptor", name);
+  FLB200_REQUIRE(d->batch >= 1 && d->q_len >= 1 && d->k_len >= d->q_len && d->heads >= 1 && d->kv_heads >= 1 &&
+                     d->heads % d->kv_heads == 0 && d->head_dim >= 1,
+                 "%s: bad extents", name);
+  FLB200_REQUIRE(d->scale > 0.f && d->scale < 1e30f, "%s: the scale must be positive", name);
+  FLB200_REQUIRE(d->softcap >= 0.f && d->softcap < 1e30f, "%s: the cap must be positive, or 0 for none", name);
+  if (!flb200_masked_attention_supported(d))
+    return fail(FLB200_UNSUPPORTED, "%s: built for f16 and bf16 and head dimensions that are multiples of 8 up to 128",
+                name);
+  return FLB200_OK;
+}
+// 16-byte rows that TMA can address
+int check_tensor(const char* name, const flb200_head_tensor* t) {
+  FLB200_REQUIRE(t && t->data, "%s: null tensor", name);
+  FLB200_REQUIRE(aligned16(t->data) && t->batch > 0 && t->row > 0 && t->head > 0 && t->batch % 8 == 0 &&
+                     t->row % 8 == 0 && t->head % 8 == 0,
+                 "%s: tensors need 16-byte aligned rows and positive strides", name);
+  return FLB200_OK;
+}
+
+template <int D, typename T, bool CAP, bool BIAS>
+int launch_forward(const flb200_attention_desc* d, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+                   AttnFwdArgs a, cudaStream_t st) {
+  const auto kernel = masked_forward_kernel<D, T, CAP, BIAS>;
+  if (int rc = configure(reinterpret_cast<const void*>(kernel), FwdSmem<D>::kTotal)) return rc;
+  a.pairs = (blocks_of(d->q_len) + 1) / 2;
+  launch_chained(kernel, (unsigned)(d->batch * d->heads * a.pairs), kThreads2, FwdSmem<D>::kTotal, st, mq, mk, mv, a);
+  FLB200_AFTER_LAUNCH("masked_attention_forward");
+  count_tc_launch();
+  return FLB200_OK;
+}
+template <int D, typename T, bool CAP, bool BIAS>
+int launch_backward(const flb200_attention_desc* d, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+                    const CUtensorMap& mg, AttnBwdArgs a, cudaStream_t st) {
+  const auto kernel = masked_backward_kernel<D, T, CAP, BIAS>;
+  if (int rc = configure(reinterpret_cast<const void*>(kernel), BwdSmem<D>::kTotal)) return rc;
+  a.kv_ctas = (int)(d->batch * d->kv_heads * blocks_of(d->k_len));
+  const unsigned grid = (unsigned)(a.kv_ctas + d->batch * d->heads * blocks_of(d->q_len));
+  launch_chained(kernel, grid, kThreads2, BwdSmem<D>::kTotal, st, mq, mk, mv, mg, a);
+  FLB200_AFTER_LAUNCH("masked_attention_backward");
+  count_tc_launch();
+  return FLB200_OK;
+}
+// f(std::integral_constant<int, D>, T, cap, bias)
+template <class F>
+int dispatch(const flb200_attention_desc* d, bool bias, const F& f) {
+  const auto by_flags = [&](auto dim, auto type) {
+    using std::false_type;
+    using std::true_type;
+    if (d->softcap > 0.f) return bias ? f(dim, type, true_type{}, true_type{}) : f(dim, type, true_type{}, false_type{});
+    return bias ? f(dim, type, false_type{}, true_type{}) : f(dim, type, false_type{}, false_type{});
+  };
+  const auto by_type = [&](auto dim) {
+    return d->dtype == FLB200_F16 ? by_flags(dim, __half{}) : by_flags(dim, __nv_bfloat16{});
+  };
+  return d->head_dim <= 64 ? by_type(std::integral_constant<int, 64>{}) : by_type(std::integral_constant<int, 128>{});
+}
+
+}  // namespace
+}  // namespace flb200
+
+using namespace flb200;
+
+extern "C" {
+
+size_t flb200_attention_mask_bytes(int64_t batch, int64_t q_len, int64_t k_len) {
+  return batch < 1 || q_len < 1 || k_len < 1 ? 0 : mask_bytes(batch, q_len, k_len);
+}
+
+int flb200_attention_mask(int64_t batch, int64_t q_len, int64_t k_len, int causal, const int32_t* documents,
+                          const int32_t* prefix, void* mask, void* stream) {
+  FLB200_REQUIRE(batch >= 1 && q_len >= 1 && k_len >= q_len && k_len < (1 << 24) && batch < 65536,
+                 "attention_mask: bad extents");
+  FLB200_REQUIRE(mask && aligned16(mask), "attention_mask: the mask must be 16-byte aligned");
+  FLB200_REQUIRE(causal || !prefix, "attention_mask: a prefix belongs to a causal mask");
+  const MaskView v = mask_view(mask, batch, q_len, k_len);
+  launch_chained(attention_mask_kernel, (unsigned)batch, 1024, 0, as_stream(stream), documents, prefix, (int)q_len,
+                 (int)k_len, causal ? 1 : 0, const_cast<int4*>(v.q_blocks), const_cast<int2*>(v.k_blocks),
+                 const_cast<int2*>(v.rows));
+  FLB200_AFTER_LAUNCH("attention_mask");
+  return FLB200_OK;
+}
+
+int flb200_masked_attention_supported(const flb200_attention_desc* d) {
+  return d && flb200_has_tensor_core_path() && (d->dtype == FLB200_BF16 || d->dtype == FLB200_F16) &&
+                 d->head_dim % 8 == 0 && d->head_dim <= 128 && d->k_len < (1 << 24) &&
+                 d->batch * d->heads * ((d->k_len + 127) / 128) < (1LL << 30)
+             ? 1
+             : 0;
+}
+
+int flb200_masked_attention_forward(const flb200_attention_desc* d, const flb200_head_tensor* q,
+                                    const flb200_head_tensor* k, const flb200_head_tensor* v, const float* slopes,
+                                    const void* mask, const flb200_head_tensor* out, float* lse, void* stream) {
+  if (int rc = check_attention("masked_attention_forward", d)) return rc;
+  FLB200_REQUIRE(mask, "masked_attention_forward: null mask");
+  for (const flb200_head_tensor* t : {q, k, v, out})
+    if (int rc = check_tensor("masked_attention_forward", t)) return rc;
+  const int operand = operand_of(d->dtype);
+  CUtensorMap mq, mk, mv;
+  if (int rc = head_map(&mq, *q, d->batch, d->heads, d->q_len, d->head_dim, operand)) return rc;
+  if (int rc = head_map(&mk, *k, d->batch, d->kv_heads, d->k_len, d->head_dim, operand)) return rc;
+  if (int rc = head_map(&mv, *v, d->batch, d->kv_heads, d->k_len, d->head_dim, operand)) return rc;
+  AttnFwdArgs a{};
+  a.s = shape_of(d, slopes, mask);
+  a.out = out_of(*out);
+  a.lse = lse;
+  return dispatch(d, slopes != nullptr, [&](auto dim, auto type, auto cap, auto bias) {
+    return launch_forward<decltype(dim)::value, decltype(type), decltype(cap)::value, decltype(bias)::value>(
+        d, mq, mk, mv, a, as_stream(stream));
+  });
+}
+
+size_t flb200_masked_attention_backward_workspace_bytes(const flb200_attention_desc* d) {
+  return !d || d->batch < 1 || d->heads < 1 || d->q_len < 1 ? 0
+                                                            : (size_t)(d->batch * d->heads * d->q_len) * sizeof(float);
+}
+
+int flb200_masked_attention_backward(const flb200_attention_desc* d, const flb200_head_tensor* q,
+                                     const flb200_head_tensor* k, const flb200_head_tensor* v,
+                                     const flb200_head_tensor* out, const flb200_head_tensor* grad_out,
+                                     const float* lse, const float* slopes, const void* mask,
+                                     const flb200_head_tensor* grad_q, const flb200_head_tensor* grad_k,
+                                     const flb200_head_tensor* grad_v, void* workspace, size_t workspace_bytes,
+                                     void* stream) {
+  if (int rc = check_attention("masked_attention_backward", d)) return rc;
+  FLB200_REQUIRE(mask && lse, "masked_attention_backward: null mask or lse");
+  for (const flb200_head_tensor* t : {q, k, v, out, grad_out, grad_q, grad_k, grad_v})
+    if (int rc = check_tensor("masked_attention_backward", t)) return rc;
+  const size_t need = flb200_masked_attention_backward_workspace_bytes(d);
+  if (!workspace || workspace_bytes < need)
+    return fail(FLB200_WORKSPACE_TOO_SMALL, "masked_attention_backward: workspace %zu < %zu", workspace_bytes, need);
+  const cudaStream_t st = as_stream(stream);
+  const int operand = operand_of(d->dtype);
+  CUtensorMap mq, mk, mv, mg;
+  if (int rc = head_map(&mq, *q, d->batch, d->heads, d->q_len, d->head_dim, operand)) return rc;
+  if (int rc = head_map(&mk, *k, d->batch, d->kv_heads, d->k_len, d->head_dim, operand)) return rc;
+  if (int rc = head_map(&mv, *v, d->batch, d->kv_heads, d->k_len, d->head_dim, operand)) return rc;
+  if (int rc = head_map(&mg, *grad_out, d->batch, d->heads, d->q_len, d->head_dim, operand)) return rc;
+  float* dsum = static_cast<float*>(workspace);
+  const long long rows = d->batch * d->heads * d->q_len;
+  const unsigned grid = (unsigned)((rows * 16 + 255) / 256);
+  if (d->dtype == FLB200_F16)
+    launch_chained(masked_dsum_kernel<__half>, grid, 256, 0, st, out_of(*out), out_of(*grad_out), dsum, rows,
+                   (int)d->q_len, (int)d->heads, (int)d->head_dim);
+  else
+    launch_chained(masked_dsum_kernel<__nv_bfloat16>, grid, 256, 0, st, out_of(*out), out_of(*grad_out), dsum, rows,
+                   (int)d->q_len, (int)d->heads, (int)d->head_dim);
+  FLB200_AFTER_LAUNCH("masked_attention_dsum");
+  AttnBwdArgs a{};
+  a.s = shape_of(d, slopes, mask);
+  a.lse = lse;
+  a.dsum = dsum;
+  a.dq = out_of(*grad_q);
+  a.dk = out_of(*grad_k);
+  a.dv = out_of(*grad_v);
+  return dispatch(d, slopes != nullptr, [&](auto dim, auto type, auto cap, auto bias) {
+    return launch_backward<decltype(dim)::value, decltype(type), decltype(cap)::value, decltype(bias)::value>(
+        d, mq, mk, mv, mg, a, st);
+  });
+}
+
+}  // extern "C"

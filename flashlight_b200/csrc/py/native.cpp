@@ -622,6 +622,130 @@ NATIVE(attention_packed_backward) {  // (qkv, out, grad_out contiguous, lse, B, 
   return wrap(g);
 }
 
+// ---------------------------------------------------------------- masked attention
+const int32_t* ints(const Tensor* t, int64_t n, const char* what) {
+  if (!t) return nullptr;
+  if (t->scalar_type() != ScalarType::Int || t->numel() != n || !t->is_contiguous() || !t->is_cuda()) {
+    PyErr_Format(PyExc_ValueError, "attention_mask: %s must be a dense int32 device tensor of %lld elements", what,
+                 (long long)n);
+    throw PyRaised();
+  }
+  return static_cast<const int32_t*>(t->data_ptr());
+}
+// (batch, q_len, k_len, causal, documents or None, prefix or None, device index) -> the mask's bytes
+NATIVE(attention_mask) {
+  const int64_t B = x.i(0), q = x.i(1), k = x.i(2);
+  if (B < 1 || q < 1 || k < q) value_error("attention_mask: batch >= 1 and 1 <= q_len <= k_len");
+  const int32_t *docs = ints(x.t(4), B * k, "documents"), *prefix = ints(x.t(5), B, "prefix");
+  Tensor m;
+  {
+    const Unlocked u;
+    m = at::detail::empty_cuda({(int64_t)flb200_attention_mask_bytes(B, q, k)}, ScalarType::Byte,
+                               at::Device(at::kCUDA, (c10::DeviceIndex)x.i(6)), std::nullopt);
+  }
+  check(unlocked(flb200_attention_mask, B, q, k, x.b(3) ? 1 : 0, docs, prefix, m.data_ptr(), stream()));
+  return wrap(m);
+}
+
+// A [batch][length][heads][head dim] tensor as the kernels take it: in place where its strides allow it, else a copy.
+struct Heads {
+  Tensor kept;
+  flb200_head_tensor h;
+  Heads(const Tensor& t, const char* what) : kept(t) {
+    if (t.dim() != 4 || !t.is_cuda()) {
+      PyErr_Format(PyExc_ValueError, "masked_attention: %s must be a device tensor (batch, length, heads, head dim)",
+                   what);
+      throw PyRaised();
+    }
+    if (!fits(t)) {
+      const Unlocked u;
+      kept = t.clone(at::MemoryFormat::Contiguous);
+    }
+    set();
+  }
+  static bool fits(const Tensor& t) {
+    bool ok = (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 && (t.stride(3) == 1 || t.size(3) == 1);
+    for (int d = 0; d < 3; ++d) ok = ok && (t.size(d) <= 1 || (t.stride(d) > 0 && t.stride(d) % 8 == 0));
+    return ok;
+  }
+  void set() {
+    const auto step = [&](int d) { return kept.size(d) > 1 ? kept.stride(d) : (kept.size(3) + 7) / 8 * 8; };
+    h = flb200_head_tensor{kept.data_ptr(), step(0), step(1), step(2)};
+  }
+};
+struct AttentionCall {
+  Heads q, k, v;
+  flb200_attention_desc d = {};
+  const float* slopes = nullptr;
+  const void* mask;
+  // args: q, k, v, slopes or None, mask, its (batch, q_len, k_len), scale, softcap
+  explicit AttentionCall(const Args& x) : q(x.tensor(0), "q"), k(x.tensor(1), "k"), v(x.tensor(2), "v") {
+    const Tensor &tq = x.tensor(0), &tk = x.tensor(1), &tv = x.tensor(2), &m = x.tensor(4);
+    const Tensor* s = x.t(3);
+    if (tk.sizes() != tv.sizes() || tq.size(0) != tk.size(0) || tq.size(3) != tk.size(3) ||
+        tq.scalar_type() != tk.scalar_type() || tq.scalar_type() != tv.scalar_type())
+      value_error("masked_attention: q, k and v must be of one type, batch and head dim, k and v alike");
+    if (tk.size(2) < 1 || tq.size(2) < 1 || tq.size(2) % tk.size(2) != 0)
+      value_error("masked_attention: the query heads must be a multiple of the key heads");
+    d.batch = x.i(5);
+    d.q_len = x.i(6);
+    d.k_len = x.i(7);
+    if (tq.size(0) != d.batch || tq.size(1) != d.q_len || tk.size(1) != d.k_len)
+      value_error("masked_attention: the mask was made for other extents");
+    d.heads = tq.size(2);
+    d.kv_heads = tk.size(2);
+    d.head_dim = tq.size(3);
+    d.scale = (float)x.d(8);
+    d.softcap = (float)x.d(9);
+    d.dtype = code_of(tq);
+    if (m.get_device() != tq.get_device()) value_error("masked_attention: the mask is on another device");
+    mask = m.data_ptr();
+    if (s) {
+      if (s->numel() != d.heads || s->scalar_type() != ScalarType::Float || !s->is_contiguous())
+        value_error("masked_attention: slopes are float32, one per query head");
+      slopes = Pf(s);
+    }
+  }
+};
+NATIVE(masked_attention) {  // (AttentionCall's) -> (out, lse)
+  AttentionCall c(x);
+  const flb200_attention_desc& d = c.d;
+  const Tensor& q = x.tensor(0);
+  Tensor out = empty({d.batch, d.q_len, d.heads, d.head_dim}, q.scalar_type(), q);
+  Tensor lse = empty({d.batch, d.heads, d.q_len}, ScalarType::Float, q);
+  const Heads o(out, "out");
+  check(unlocked(flb200_masked_attention_forward, &d, (const flb200_head_tensor*)&c.q.h,
+                 (const flb200_head_tensor*)&c.k.h, (const flb200_head_tensor*)&c.v.h, c.slopes, c.mask, &o.h, Pf(&lse),
+                 stream()));
+  return wrap({out, lse});
+}
+// (AttentionCall's, out, grad_out, lse, grad_q, grad_k, grad_v or None three times: new tensors) -> (grad_q, ...)
+NATIVE(masked_attention_backward) {
+  AttentionCall c(x);
+  const flb200_attention_desc& d = c.d;
+  const Tensor &out = x.tensor(10), &gy = x.tensor(11), &lse = x.tensor(12);
+  if (out.sizes() != x.tensor(0).sizes() || gy.sizes() != out.sizes() || gy.scalar_type() != out.scalar_type() ||
+      out.scalar_type() != x.tensor(0).scalar_type())
+    value_error("masked_attention: the output's gradient must be like the output");
+  if (lse.numel() != d.batch * d.heads * d.q_len || lse.scalar_type() != ScalarType::Float)
+    value_error("masked_attention: lse does not belong to these tensors");
+  const Heads o(out, "out"), g(gy, "grad_out");
+  Tensor grads[3];
+  for (int i = 0; i < 3; ++i) {
+    const Tensor& like = x.tensor(i);
+    const Tensor* given = x.t(13 + i);
+    if (given && (given->sizes() != like.sizes() || given->scalar_type() != like.scalar_type() || !Heads::fits(*given)))
+      value_error("masked_attention: a given gradient must be like its tensor, in aligned rows");
+    grads[i] = given ? *given : empty(like.sizes(), like.scalar_type(), like);
+  }
+  const Heads gq(grads[0], "grad_q"), gk(grads[1], "grad_k"), gv(grads[2], "grad_v");
+  Workspace ws(flb200_masked_attention_backward_workspace_bytes(&d), out);
+  check(unlocked(flb200_masked_attention_backward, &d, (const flb200_head_tensor*)&c.q.h,
+                 (const flb200_head_tensor*)&c.k.h, (const flb200_head_tensor*)&c.v.h, &o.h, &g.h,
+                 (const float*)Pf(&lse), c.slopes, c.mask, &gq.h, &gk.h, &gv.h, ws.p(), ws.bytes, stream()));
+  return wrap({grads[0], grads[1], grads[2]});
+}
+
 // ---------------------------------------------------------------- embedding
 int id_code(const Tensor& ids) {
   if (ids.scalar_type() == ScalarType::Long) return FLB200_IDS_I64;
@@ -1069,7 +1193,8 @@ NATIVE(set_check) {  // (callable)
 
 #define ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
-    ENTRY(set_check), ENTRY(adamw_step), ENTRY(linear_cce_forward), ENTRY(linear_cce_backward), ENTRY(unary), ENTRY(binary), ENTRY(relu_mask), ENTRY(relu_mask_backward),
+    ENTRY(set_check), ENTRY(adamw_step), ENTRY(attention_mask), ENTRY(masked_attention), ENTRY(masked_attention_backward),
+    ENTRY(linear_cce_forward), ENTRY(linear_cce_backward), ENTRY(unary), ENTRY(binary), ENTRY(relu_mask), ENTRY(relu_mask_backward),
     ENTRY(dropout_apply), ENTRY(astype), ENTRY(reorder), ENTRY(bernoulli_mask), ENTRY(channel_sum),
     ENTRY(channel_bias_add), ENTRY(layernorm), ENTRY(layernorm_backward), ENTRY(linear),
     ENTRY(linear_bias_act), ENTRY(linear_backward), ENTRY(matmul), ENTRY(log_softmax),

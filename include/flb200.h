@@ -594,6 +594,51 @@ int flb200_attention_packed_backward(const void* qkv, const void* out, const voi
                                      int64_t seq_len, int64_t head_dim, float scale, int causal, int dtype,
                                      void* workspace, size_t workspace_bytes, void* stream);
 
+/* Attention (Functions.cpp:1828-1891) where each query sees an interval of the keys.  Query i of q_len stands at
+ * position i + k_len - q_len (q_len <= k_len: the last positions, down to a single one).
+ *
+ * The mask is made once per batch, on the device, and serves every layer and both directions.  documents (int32
+ * [batch][k_len], or NULL): a position sees those of its own run of equal ids; ids below zero are padding, which
+ * sees nothing and, by that rule, is seen by nobody else's run.  causal: position p sees p and what is before
+ * it.  prefix (int32 [batch], or NULL; with causal): the row's first prefix positions are seen by all (of their
+ * document).  A query that sees nothing has zeros for its output and minus infinity for its lse. */
+size_t flb200_attention_mask_bytes(int64_t batch, int64_t q_len, int64_t k_len);
+int flb200_attention_mask(int64_t batch, int64_t q_len, int64_t k_len, int causal, const int32_t* documents,
+                          const int32_t* prefix, void* mask, void* stream);
+
+/* out = softmax(s) v with  s = softcap * tanh(scale q.k / softcap) - slopes[head] * |i - j|  over the keys that the
+ * mask leaves; softcap 0: s = scale q.k - ..., slopes (fp32 [heads], a constant: it takes no gradient) may be NULL.
+ * Query head h reads key head h / (heads / kv_heads).  FLB200_F16 or FLB200_BF16, head_dim a multiple of 8 up to
+ * 128 (flb200_masked_attention_supported; else FLB200_UNSUPPORTED); scores, statistics and sums are fp32, the
+ * probabilities and the scores' gradient are rounded to the tensors' type as operands.  Tensors by strides in
+ * elements, each a multiple of 8, data 16-byte aligned: element (b, t, h, d) at b*batch + t*row + h*head + d.
+ * The values of k and v in a block of 128 positions that some query of a block sees must be finite, or that
+ * query block's output is not.  lse: fp32 [batch][heads][q_len] (NULL in forward: not kept).
+ * Backward gives the gradients of q, k and v (those of k and v summed over the heads that share them), without
+ * atomics: equal inputs give equal bits. */
+typedef struct flb200_attention_desc {
+  int64_t batch, q_len, k_len, heads, kv_heads, head_dim;
+  float scale, softcap;
+  int32_t dtype;
+} flb200_attention_desc;
+typedef struct flb200_head_tensor {
+  void* data;
+  int64_t batch, row, head; /* strides */
+} flb200_head_tensor;
+int flb200_masked_attention_supported(const flb200_attention_desc* d);
+int flb200_masked_attention_forward(const flb200_attention_desc* d, const flb200_head_tensor* q,
+                                    const flb200_head_tensor* k, const flb200_head_tensor* v,
+                                    const float* slopes, const void* mask, const flb200_head_tensor* out,
+                                    float* lse, void* stream);
+size_t flb200_masked_attention_backward_workspace_bytes(const flb200_attention_desc* d);
+int flb200_masked_attention_backward(const flb200_attention_desc* d, const flb200_head_tensor* q,
+                                     const flb200_head_tensor* k, const flb200_head_tensor* v,
+                                     const flb200_head_tensor* out, const flb200_head_tensor* grad_out,
+                                     const float* lse, const float* slopes, const void* mask,
+                                     const flb200_head_tensor* grad_q, const flb200_head_tensor* grad_k,
+                                     const flb200_head_tensor* grad_v, void* workspace, size_t workspace_bytes,
+                                     void* stream);
+
 /* logSoftmax over fl dim 0: x, y [C, X] column-major (Functions.cpp:1044-1070). */
 int flb200_log_softmax_forward(const void* x, void* y, int64_t C, int64_t X, int dtype,
                                void* stream);
