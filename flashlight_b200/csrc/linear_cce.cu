@@ -31,11 +31,14 @@ namespace {
 
 using namespace tc;
 
-__device__ __forceinline__ float exp_below(float x) {  // e^x, x being a difference from a row's maximum or lse
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float exp2_of(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// e^x, x being a difference from a row's maximum
+__device__ __forceinline__ float exp_below(float x) { return exp2_of(x * kLog2e); }
 // element (row r, column c) of an epilogue warp's staged 32 x 32 chunk (epi_stage_write)
 __device__ __forceinline__ float staged(const float* stage, int r, int c) {
   return stage[r * 32 + (((c >> 2) ^ (r & 7)) << 2) + (c & 3)];
@@ -78,8 +81,7 @@ struct ScoreArgs {
   int col0;
   float* target_score;     // forward: [M]
   float2* partial;         // forward: (maximum, sum) [tiles * groups of this piece][M]
-  const float* lse;        // gradient
-  const float* weight;     // gradient: [M], what G is stored with; 0 where the row does not count
+  const struct RowInfo* rows;  // gradient: [M]
   void* grad;              // gradient: [M][grad_ld] of T
   long long grad_ld;
   float* column_sum;       // gradient: [groups of 32 rows][grad_ld], or null
@@ -154,6 +156,16 @@ struct LseProblem : ScoreProblem<BN> {
   }
 };
 
+// What a row of the gradient's scores needs, one 16-byte load: lse log2 e, what G is stored with (0 where the row does
+// not count) and the target.
+struct RowInfo {
+  float lse_log2, weight;
+  int target, unused;
+};
+
+// A lane has 32 columns of its row, 64 bytes of G: it stores them itself, whole sectors of 32 bytes.  Only the
+// columns' sums pass through the staging tile.  (Staged like the other products' results, with three loads per row
+// and a test per element, a tile of 256 columns took 16700 clocks, two and a half times its contraction over 768.)
 template <int BN, typename T>
 struct GradScoreProblem : ScoreProblem<BN> {
   __device__ __forceinline__ void store(const typename GemmProblem<BN>::Tile& t, int row, int c0, const float* v,
@@ -161,29 +173,75 @@ struct GradScoreProblem : ScoreProblem<BN> {
     const int m = t.m0 + row, nb = t.n0 + c0, m_first = m - lane;
     const ScoreArgs& s = this->s;
     if (m_first >= this->M) return;  // (the whole warp)
-    float z[32];
-    this->add_bias(nb, v, z);
-    float weight = 0.f, lse = 0.f;
-    int rel = -1;
+    RowInfo info{0.f, 0.f, -1, 0};
     if (m < this->M) {
-      weight = s.weight[m];
-      lse = s.lse[m];
-      rel = s.targets[m] - s.col0 - nb;
+      const int4 r = __ldg(reinterpret_cast<const int4*>(s.rows + m));
+      info = RowInfo{__int_as_float(r.x), __int_as_float(r.y), r.z, 0};
     }
-    // (a row that does not count is zeros whatever its scores)
+    const float less = -info.lse_log2;
+    float z[32];
+    if (!s.bias) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) z[j] = weight == 0.f ? 0.f : weight * exp_below(z[j] - lse);
+      for (int j = 0; j < 32; ++j) z[j] = fmaf(v[j], kLog2e, less);
+    } else if (s.bias_vec && nb + 32 <= this->N) {
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) {
+        const float4 b = __ldg(reinterpret_cast<const float4*>(s.bias + nb + j));
+        z[j] = fmaf(v[j] + b.x, kLog2e, less);
+        z[j + 1] = fmaf(v[j + 1] + b.y, kLog2e, less);
+        z[j + 2] = fmaf(v[j + 2] + b.z, kLog2e, less);
+        z[j + 3] = fmaf(v[j + 3] + b.w, kLog2e, less);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        z[j] = fmaf(nb + j < this->N ? v[j] + __ldg(s.bias + nb + j) : v[j], kLog2e, less);
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) z[j] = info.weight * exp2_of(z[j]);
+    if (info.weight == 0.f) {  // zeros whatever the row's scores
+#pragma unroll
+      for (int j = 0; j < 32; ++j) z[j] = 0.f;
+    }
+    const int rel = info.target - s.col0 - nb;
     if (rel >= 0 && rel < 32) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) z[j] = j == rel ? z[j] - weight : z[j];
+      for (int j = 0; j < 32; ++j) z[j] = j == rel ? z[j] - info.weight : z[j];
     }
-    epi_stage_write(stage, lane, z);
-    store_staged<T, false>(stage, lane, static_cast<T*>(s.grad), s.grad_ld, m_first, this->M, nb, this->N, true);
-    if (s.column_sum) {  // of the chunk's rows (those past the end are zeros), a column per lane
-      float sum = 0.f;
+    const bool whole = nb + 32 <= this->N;
+    T* out = static_cast<T*>(s.grad);
+    if (whole && m < this->M) {
+      T* to = out + (long long)m * s.grad_ld + nb;
 #pragma unroll
-      for (int r = 0; r < 32; ++r) sum += staged(stage, r, lane);
-      if (nb + lane < this->N) s.column_sum[(long long)(m_first >> 5) * s.grad_ld + nb + lane] = sum;
+      for (int j = 0; j < 32; j += 16) {
+        const Vec16<T> lo = pack16<T>(z + j), hi = pack16<T>(z + j + 8);
+        const uint4 a = *reinterpret_cast<const uint4*>(&lo), b = *reinterpret_cast<const uint4*>(&hi);
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + j), "r"(a.x), "r"(a.y),
+                     "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+                     : "memory");
+      }
+    }
+    if (whole && !s.column_sum) return;
+    epi_stage_write(stage, lane, z);
+    if (!whole)
+      store_staged<T, false>(stage, lane, out, s.grad_ld, m_first, this->M, nb, this->N, true);
+    if (s.column_sum) {
+      // four columns of every fourth row, then the four lanes that have the same columns; rows past the end are zeros
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float4 x = epi_stage_read(stage, lane, k);
+        sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+      }
+#pragma unroll
+      for (int o = 8; o < 32; o <<= 1) {
+        sum.x += __shfl_xor_sync(0xffffffffu, sum.x, o);
+        sum.y += __shfl_xor_sync(0xffffffffu, sum.y, o);
+        sum.z += __shfl_xor_sync(0xffffffffu, sum.z, o);
+        sum.w += __shfl_xor_sync(0xffffffffu, sum.w, o);
+      }
+      if (lane < 8)  // (rows of sums are as long as whole chunks)
+        *reinterpret_cast<float4*>(s.column_sum + (long long)(m_first >> 5) * s.grad_ld + nb + 4 * lane) = sum;
     }
     __syncwarp();  // the staging tile is rewritten by the next chunk
   }
@@ -293,9 +351,9 @@ __device__ __forceinline__ bool counts(int target, int ignore, long long classes
   return target != ignore && target >= 0 && target < classes;
 }
 
-// Joins the tiles' (maximum, sum) of 32 rows per CTA: eight threads to a row take every eighth part and meet in shared
-// memory.  Then the rows' losses, and their sum and count per CTA.
-constexpr int kJoin = 8;
+// Joins the tiles' (maximum, sum) of 32 rows per CTA: 32 threads to a row take every 32nd part and meet in shared
+// memory (with eight to a row 13 us for 4096 rows of 250 parts).  Then the rows' losses, and their sum and count per CTA.
+constexpr int kJoin = 32;
 __global__ void __launch_bounds__(32 * kJoin)
 join_lse_kernel(const float2* __restrict__ partial, int parts, const float* __restrict__ target_score,
                 const int32_t* __restrict__ targets, int ignore, long long classes, int rows,
@@ -315,15 +373,17 @@ join_lse_kernel(const float2* __restrict__ partial, int parts, const float* __re
     }
   }
   met[g][lane] = make_float2(top, sum);
-  __syncthreads();
-  if (g > 0) return;
-#pragma unroll
-  for (int k = 1; k < kJoin; ++k) {
-    const float2 x = met[k][lane];
-    const float mx = fmaxf(top, x.x);
-    sum = sum * exp_below(top - mx) + x.y * exp_below(x.x - mx);
-    top = mx;
+  for (int half = kJoin / 2; half > 0; half >>= 1) {
+    __syncthreads();
+    if (g < half) {
+      const float2 x = met[g + half][lane];
+      const float mx = fmaxf(top, x.x);
+      sum = sum * exp_below(top - mx) + x.y * exp_below(x.x - mx);
+      top = mx;
+      met[g][lane] = make_float2(top, sum);
+    }
   }
+  if (g > 0) return;
   double loss = 0.0, n = 0.0;
   if (r < rows) {
     const float l = top + logf(sum);
@@ -362,11 +422,12 @@ finish_loss_kernel(const double2* __restrict__ sums, int n, float* __restrict__ 
   }
 }
 
-// weight[r] = step * g_r / max |g|, zero where the row does not count; factor = max |g| / step
+// Each row's RowInfo, its weight step * g_r / max |g|, zero where the row does not count; factor = max |g| / step
 __global__ void __launch_bounds__(1024)
 row_weights_kernel(const float* __restrict__ grad_loss, const int32_t* __restrict__ targets,
-                   const int32_t* __restrict__ count, int reduction, int ignore, long long classes, int rows,
-                   float step, float* __restrict__ weight, float* __restrict__ factor) {
+                   const int32_t* __restrict__ count, const float* __restrict__ lse, int reduction, int ignore,
+                   long long classes, int rows, float step, RowInfo* __restrict__ info,
+                   float* __restrict__ factor) {
   chain_begin();
   __shared__ float scratch[32];
   float top = 0.f;
@@ -386,7 +447,7 @@ row_weights_kernel(const float* __restrict__ grad_loss, const int32_t* __restric
     float w = 0.f;
     if (counts(targets[r], ignore, classes))
       w = reduction != FLB200_REDUCE_NONE ? step : (top > 0.f ? step * (grad_loss[r] / top) : 0.f);
-    weight[r] = w;
+    info[r] = RowInfo{lse[r] * kLog2e, w, targets[r], 0};
   }
 }
 
@@ -499,11 +560,12 @@ int fit_splits(long long K, int splits, int* stages_each) {
   return (int)((stages + each - 1) / each);
 }
 struct BackwardScratch {
-  float *weight, *factor, *dx, *column_sum;
+  RowInfo* rows;
+  float *factor, *dx, *column_sum;
   uint16_t *grad, *x, *w;
   int dx_splits;
   BackwardScratch(Carve& c, const Shape& s, bool need_x, bool need_bias) {
-    weight = c.take<float>(s.rows);
+    rows = c.take<RowInfo>(s.rows);
     factor = c.take<float>(1);
     grad = c.take<uint16_t>(s.rows * s.piece);
     int stages;
@@ -643,8 +705,8 @@ int flb200_linear_cce_backward(const flb200_linear_cce_desc* d, const void* x, c
   Carve carve{static_cast<char*>(workspace)};
   const BackwardScratch scratch(carve, s, true, true);
   const bool bf16 = d->dtype == FLB200_BF16;
-  launch_chained(row_weights_kernel, 1, 1024, 0, st, grad_loss, targets, count, d->reduction, d->ignore_index,
-                 s.classes, (int)s.rows, bf16 ? 1.f : 32768.f, scratch.weight, scratch.factor);
+  launch_chained(row_weights_kernel, 1, 1024, 0, st, grad_loss, targets, count, lse, d->reduction, d->ignore_index,
+                 s.classes, (int)s.rows, bf16 ? 1.f : 32768.f, scratch.rows, scratch.factor);
   FLB200_AFTER_LAUNCH("linear_cce_weights");
   for (long long col0 = 0; col0 < s.classes; col0 += s.piece) {
     const long long cols = std::min(s.piece, s.classes - col0);
@@ -657,8 +719,7 @@ int flb200_linear_cce_backward(const flb200_linear_cce_desc* d, const void* x, c
     a.bias_vec = bias && aligned16(bias);
     a.targets = targets;
     a.col0 = (int)col0;
-    a.lse = lse;
-    a.weight = scratch.weight;
+    a.rows = scratch.rows;
     a.grad = scratch.grad;
     a.grad_ld = s.piece;
     a.column_sum = grad_bias ? scratch.column_sum : nullptr;
