@@ -20,6 +20,7 @@
 #include <cmath>
 
 #include "common.cuh"
+#include "packed.cuh"
 
 namespace flb200 {
 namespace {
@@ -78,36 +79,6 @@ __device__ __forceinline__ void store8(T* p, bool whole, int live, const float* 
   }
 }
 
-// Two fp32 numbers in one register pair: one instruction for both, each rounded as it would be alone.
-struct F2 {
-  unsigned long long r;
-};
-__device__ __forceinline__ F2 pair(float a, float b) {
-  F2 x;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(x.r) : "f"(a), "f"(b));
-  return x;
-}
-__device__ __forceinline__ void unpair(F2 x, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.r));
-}
-__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
-  F2 x;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(x.r) : "l"(a.r), "l"(b.r));
-  return x;
-}
-// One by one: the assembler makes one rounding of a paired product and the paired sum behind it.
-__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
-  float a0, a1, b0, b1;
-  unpair(a, a0, a1);
-  unpair(b, b0, b1);
-  return pair(__fadd_rn(a0, b0), __fadd_rn(a1, b1));
-}
-__device__ __forceinline__ F2 fused(F2 a, F2 b, F2 c) {
-  F2 x;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x.r) : "l"(a.r), "l"(b.r), "l"(c.r));
-  return x;
-}
-
 // 8-bit states: eight codes, their values over the block's scale
 __device__ __forceinline__ void load_codes(const uint8_t* p, bool whole, int live, float scale, float* v) {
   uint32_t w[2] = {0, 0};
@@ -120,7 +91,7 @@ __device__ __forceinline__ void load_codes(const uint8_t* p, bool whole, int liv
     for (int j = 0; j < kPer; ++j)
       if (j < live) w[j >> 2] |= (uint32_t)p[j] << (8 * (j & 3));
   }
-  const F2 s = pair(scale, scale);
+  const F2 s = pair(scale);
 #pragma unroll
   for (int j = 0; j < kPer; j += 2) {
     const __half2_raw h =
@@ -137,7 +108,7 @@ __device__ __forceinline__ void store_codes(uint8_t* p, float* scale, bool whole
   for (int j = 0; j < kPer; ++j) top = fmaxf(top, kRoot ? v[j] : fabsf(v[j]));  // (past the end: zeros)
   top = fmaxf(warp_max(top), 1e-30f);
   const float to_code = __fmul_rn(__frcp_rn(top), 448.f);
-  const F2 k = pair(to_code, to_code);
+  const F2 k = pair(to_code);
   uint32_t w[2] = {0, 0};
 #pragma unroll
   for (int j = 0; j < kPer; j += 2) {
@@ -196,19 +167,19 @@ adamw_kernel(const __grid_constant__ AdamwTable<CAP> table, const AdamwMath k) {
     // the formula alone.
 #pragma unroll
     for (int j = 0; j < kPer; j += 2) {
-      const F2 gg = pair(g[j], g[j + 1]) * pair(k.grad_scale, k.grad_scale);
-      const F2 mm = pair(m[j], m[j + 1]) * pair(k.beta1, k.beta1) + gg * pair(k.rest1, k.rest1);
+      const F2 gg = pair(g[j], g[j + 1]) * pair(k.grad_scale);
+      const F2 mm = add_apart(pair(m[j], m[j + 1]) * pair(k.beta1), gg * pair(k.rest1));
       F2 vv = pair(v[j], v[j + 1]);
       if (BITS == 8) vv = vv * vv;
-      vv = vv * pair(k.beta2, k.beta2) + gg * gg * pair(k.rest2, k.rest2);
+      vv = add_apart(vv * pair(k.beta2), gg * gg * pair(k.rest2));
       float v0, v1, d0, d1, u0, u1;
       unpair(vv, v0, v1);
       const float r0 = __fsqrt_rn(v0), r1 = __fsqrt_rn(v1);
-      unpair(fused(pair(r0, r1), pair(k.inv_root_c2, k.inv_root_c2), pair(k.epsilon, k.epsilon)), d0, d1);
-      unpair(mm * pair(k.inv_c1, k.inv_c1), u0, u1);
+      unpair(fused(pair(r0, r1), pair(k.inv_root_c2), pair(k.epsilon)), d0, d1);
+      unpair(mm * pair(k.inv_c1), u0, u1);
       const F2 pp = pair(p[j], p[j + 1]);
-      const F2 step = fused(pp, pair(k.weight_decay, k.weight_decay), pair(__fdividef(u0, d0), __fdividef(u1, d1)));
-      unpair(fused(step, pair(-k.lr, -k.lr), pp), p[j], p[j + 1]);
+      const F2 step = fused(pp, pair(k.weight_decay), pair(__fdividef(u0, d0), __fdividef(u1, d1)));
+      unpair(fused(step, pair(-k.lr), pp), p[j], p[j + 1]);
       unpair(mm, m[j], m[j + 1]);
       v[j] = BITS == 32 ? v0 : r0;
       v[j + 1] = BITS == 32 ? v1 : r1;

@@ -23,6 +23,7 @@
 
 #include "common.cuh"
 #include "flb200.h"
+#include "packed.cuh"
 #include "tc_core.cuh"
 #include "tc_gemm.cuh"
 
@@ -623,7 +624,7 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 template <int D>
 struct BwdSmem {
   static constexpr int kTile = D / 64 * kBox, kStages = 2;
-  static constexpr int kColumns = 2 * 128 * 16;  // two buffers of (lse, D, lo, hi) per query column
+  static constexpr int kColumns = 2 * 128 * 16;  // two buffers of lse and D, and of the interval, per query column
   static constexpr int kTotal = 2 * kTile + 2 * kStages * kTile + kColumns + 1024 + 256;
 };
 struct AttnBwdArgs {
@@ -643,8 +644,9 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
   extern __shared__ __align__(1024) char smem_raw[];
   char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   char *sR1 = base, *sR2 = base + kTile, *sC1 = base + 2 * kTile, *sC2 = sC1 + kStages * kTile;
-  float4* columns = reinterpret_cast<float4*>(sC2 + kStages * kTile);  // [2][128]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(columns + 256);
+  float2* columns = reinterpret_cast<float2*>(sC2 + kStages * kTile);  // [2][128] lse, D
+  int2* intervals = reinterpret_cast<int2*>(columns + 256);            // [2][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(intervals + 256);
   uint64_t *bar_r = bars, *full = bars + 1, *empty = full + kStages, *bar_s = empty + kStages, *bar_p = bar_s + 2,
            *bar_a = bar_p + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_a + 1);
@@ -775,23 +777,31 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
     }
     if (BIAS && !KV) slope = a.s.slopes[head] * kLog2e;
     // of a query block's columns: lse, D and the interval, a thread per column
+    struct Column { float2 ld; int2 seen; };
     auto column = [&](int in_head, int hq) {
-      float4 c = make_float4(INFINITY, 0.f, 0.f, 0.f);
+      Column c{make_float2(INFINITY, 0.f), make_int2(0, 0)};
       const int q = (first + in_head) * kBlock + 64 * h + tid;
       if (tid < 64 && q < a.s.q_len) {
-        const int2 r = a.s.mask.rows[(long long)batch * a.s.q_len + q];
-        c = make_float4(lse_of(rows0 + (long long)hq * a.s.q_len + q), a.dsum[rows0 + (long long)hq * a.s.q_len + q],
-                        __int_as_float(r.x), __int_as_float(r.y));
+        const long long at = rows0 + (long long)hq * a.s.q_len + q;
+        c.seen = a.s.mask.rows[(long long)batch * a.s.q_len + q];
+        c.ld = make_float2(lse_of(at), a.dsum[at]);
       }
       return c;
     };
-    if (KV && total > 0 && tid < 64) columns[64 * h + tid] = column(0, 0);
+    auto keep = [&](int buffer, const Column& c) {
+      if (tid < 64) {
+        columns[buffer * 128 + 64 * h + tid] = c.ld;
+        intervals[buffer * 128 + 64 * h + tid] = c.seen;
+      }
+    };
+    if (KV && total > 0) keep(0, column(0, 0));
     int in_head = 0, hq = 0;
     for (int it = 0; it < total; ++it) {
       const int col0 = (first + in_head) * kBlock + 64 * h;  // first column of this half
-      const float4* cols = columns + (it & 1) * 128 + 64 * h;
+      const float2* cols = columns + (it & 1) * 128 + 64 * h;
+      const int2* seen_by = intervals + (it & 1) * 128 + 64 * h;
       bool whole;
-      float4 ahead;
+      Column ahead;
       int next_in = in_head + 1, next_hq = hq;
       if (next_in == count) { next_in = 0; ++next_hq; }
       if (KV) {
@@ -815,35 +825,53 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
         settle(sr);
         settle(dr);
         uint32_t p[16], ds[16];
+        // two columns at a time; `whole` tests no element
+        const auto columns_of = [&](auto tested) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float p2[2], ds2[2];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int col = 32 * c + e + k;
-            float4 x;
-            if (KV) x = cols[col];
-            float lse = KV ? x.x : my_lse, z = __uint_as_float(sr[e + k]), flat = 1.f;
-            if (BIAS) lse = fmaf(slope, fabsf(apart - (float)col), lse);
+          for (int e = 0; e < 32; e += 2) {
+            const int col = 32 * c + e;
+            float4 x;  // lse and D of both columns
+            if (KV) x = *reinterpret_cast<const float4*>(cols + col);
+            F2 less = KV ? pair(-x.x, -x.z) : pair(-my_lse);
+            if (BIAS)
+              less = fused(pair(fabsf(apart - (float)col), fabsf(apart - (float)(col + 1))), pair(-slope), less);
+            F2 z = pair(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1])), flat;
             if (CAP) {
-              const float r = rcp(1.f + ex2(z * a.s.to_2u_log2));
-              z = fmaf(-2.f * a.s.cap_log2, r, a.s.cap_log2) - lse;
-              flat = 4.f * fmaf(-r, r, r);
+              float z0, z1;
+              unpair(z * pair(a.s.to_2u_log2), z0, z1);
+              const F2 r = pair(rcp(1.f + ex2(z0)), rcp(1.f + ex2(z1)));
+              z = fused(r, pair(-2.f * a.s.cap_log2), pair(a.s.cap_log2)) + less;
+              flat = r * fused(r, pair(-4.f), pair(4.f));
             } else {
-              z = fmaf(z, a.s.to_log2, -lse);
+              z = fused(z, pair(a.s.to_log2), less);
             }
-            p2[k] = ex2(z);
-            ds2[k] = p2[k] * (__uint_as_float(dr[e + k]) - (KV ? x.y : my_d));
-            if (CAP) ds2[k] *= flat;
-            if (!whole) {  // what is not seen counts nothing, whatever its score
-              const bool sees = KV ? mine >= __float_as_int(x.z) && mine < __float_as_int(x.w)
-                                   : col0 + col >= seen.x && col0 + col < seen.y;
-              if (!sees) p2[k] = ds2[k] = 0.f;
+            float p0, p1, d0, d1;
+            unpair(z, p0, p1);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            F2 d = pair(__uint_as_float(dr[e]), __uint_as_float(dr[e + 1])) + (KV ? pair(-x.y, -x.w) : pair(-my_d));
+            d = d * pair(p0, p1);
+            if (CAP) d = d * flat;
+            unpair(d, d0, d1);
+            if constexpr (decltype(tested)::value) {  // what is not seen counts nothing, whatever its score
+              bool sees0, sees1;
+              if (KV) {
+                const int4 r = *reinterpret_cast<const int4*>(seen_by + col);
+                sees0 = mine >= r.x && mine < r.y;
+                sees1 = mine >= r.z && mine < r.w;
+              } else {
+                sees0 = col0 + col >= seen.x && col0 + col < seen.y;
+                sees1 = col0 + col + 1 >= seen.x && col0 + col + 1 < seen.y;
+              }
+              if (!sees0) p0 = d0 = 0.f;
+              if (!sees1) p1 = d1 = 0.f;
             }
+            p[e / 2] = pack2<T>(p0, p1);
+            ds[e / 2] = pack2<T>(d0, d1);
           }
-          p[e / 2] = pack2<T>(p2[0], p2[1]);
-          ds[e / 2] = pack2<T>(ds2[0], ds2[1]);
-        }
+        };
+        if (whole) columns_of(std::false_type{});
+        else columns_of(std::true_type{});
         if (KV) st16(s_addr + 16 * c, p);
         st16(s_addr + 64 + 16 * c, ds);
       }
@@ -852,7 +880,7 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
       __syncwarp();
       if (lane == 0) arrive(&bar_p[h]);
       // (the other buffer was last read before this block's barrier)
-      if (KV && it + 1 < total && tid < 64) columns[((it + 1) & 1) * 128 + 64 * h + tid] = ahead;
+      if (KV && it + 1 < total) keep((it + 1) & 1, ahead);
       in_head = next_in;
       hq = next_hq;
     }
