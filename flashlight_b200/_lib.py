@@ -167,9 +167,10 @@ SIGNATURES = {
     "flb200_attention_mask": (C.c_int, [i64, i64, i64, C.c_int, vp, vp, vp, vp]),
     "flb200_masked_attention_supported": (C.c_int, [P(AttentionDesc)]),
     "flb200_masked_attention_forward": (C.c_int, [P(AttentionDesc), P(HeadTensor), P(HeadTensor), P(HeadTensor),
-                                                  vp, vp, P(HeadTensor), vp, vp]),
+                                                  vp, vp, P(HeadTensor), vp, vp, vp]),
     "flb200_masked_attention_backward_workspace_bytes": (sz, [P(AttentionDesc)]),
-    "flb200_masked_attention_backward": (C.c_int, [P(AttentionDesc)] + [P(HeadTensor)] * 5 + [vp, vp, vp] +
+    "flb200_masked_attention_backward": (C.c_int, [P(AttentionDesc)] + [P(HeadTensor)] * 4 +
+                                         [vp, P(HeadTensor), vp, vp, vp] +
                                          [P(HeadTensor)] * 3 + [vp, sz, vp]),
     "flb200_sgd_step": (C.c_int, [vp, vp, vp, i64, f32, f32, f32, C.c_int, f32, C.c_int, C.c_int, vp]),
     "flb200_adamw_step": (C.c_int, [P(AdamwDesc), P(AdamwTensor), i64, vp]),

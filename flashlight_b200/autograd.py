@@ -738,13 +738,15 @@ def masked_attention(q: Variable, k: Variable, v: Variable, mask: F.AttentionMas
                      softcap: float = 0.0, slopes: Optional[torch.Tensor] = None) -> Variable:
     """softmax(softcap * tanh(scale q k^T / softcap) - slopes |i - j|) v where each query sees an interval of the
     keys (functions.attention_mask: causal, documents of a packed row, a prefix): q (batch, length, heads, head
-    dim), k and v with as many heads or a divisor of them.  One kernel forward, which keeps the rows' log-sum-exp,
-    and one for the three gradients behind a small pass over the output's.  slopes take no gradient."""
+    dim), k and v with as many heads or a divisor of them.  One kernel forward, which for the gradient keeps the
+    rows' log-sum-exp and what the output's rounding took, and one for the three gradients behind a small pass
+    over the output's.  slopes take no gradient."""
     qt, kt, vt = q.tensor, k.tensor, v.tensor
-    out, lse = F.masked_attention(qt, kt, vt, mask, scale, softcap, slopes)
+    train = q.isCalcGrad() or k.isCalcGrad() or v.isCalcGrad()
+    out, lse, rest = F.masked_attention(qt, kt, vt, mask, scale, softcap, slopes, train)
 
     def grad_func(inputs, gy):
-        grads = F.masked_attention_backward(qt, kt, vt, out, gy, lse, mask, scale, softcap, slopes)
+        grads = F.masked_attention_backward(qt, kt, vt, out, rest, gy, lse, mask, scale, softcap, slopes)
         for inp, g in zip(inputs, grads):
             inp.addGrad(g)
 
@@ -766,11 +768,12 @@ def masked_attention_packed(qkv: Variable, heads: int, mask: F.AttentionMask, sc
         x = x.view(B, T, heads + 2 * kv_heads, hd)
         return x[:, :, :heads], x[:, :, heads:heads + kv_heads], x[:, :, heads + kv_heads:]
 
-    out, lse = F.masked_attention(*parts(t), mask, scale, softcap, slopes)
+    out, lse, rest = F.masked_attention(*parts(t), mask, scale, softcap, slopes, qkv.isCalcGrad())
 
     def grad_func(inputs, gy):
         g = torch.empty_like(t)
-        F.masked_attention_backward(*parts(t), out, gy.reshape(out.shape), lse, mask, scale, softcap, slopes, parts(g))
+        F.masked_attention_backward(*parts(t), out, rest, gy.reshape(out.shape), lse, mask, scale, softcap, slopes,
+                                    parts(g))
         inputs[0].addGrad(g)
 
     return Variable(out.view(B * T, heads * hd), False, [qkv], grad_func)

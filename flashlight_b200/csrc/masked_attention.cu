@@ -35,7 +35,7 @@ using namespace tc;
 constexpr int kBlock = 128;        // queries and keys of a block
 constexpr int kBox = 128 * 128;    // bytes of [128 rows][64 16-bit values], one TMA box
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kThreads2 = 320;     // warps 0..7: two threads per row or a tile each; 8: TMA; 9: MMA
+constexpr int kThreads2 = 320;     // warps 0..7: two threads per row; 8: TMA; 9: MMA
 
 // ------------------------------------------------------------------------------------------ the mask
 // rows: [lo, hi) of each query ([batch][q_len]; hi <= lo: it sees nothing).  q_blocks: of each block of queries the
@@ -242,16 +242,20 @@ __device__ __forceinline__ void ld32_begin(uint32_t addr, uint32_t* r) {
 }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void settle(uint32_t* r) { asm volatile("" : FLB200_R32(r)); }
-__device__ __forceinline__ void st32(uint32_t addr, const uint32_t* r) {
+__device__ __forceinline__ void ld16_begin(uint32_t addr, uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
       : "memory");
+}
+__device__ __forceinline__ void settle16(uint32_t* r) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15]));
 }
 __device__ __forceinline__ void st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
@@ -298,18 +302,28 @@ struct OutTensor {  // element (batch b, row t, head h, d) at b * batch + t * ro
   void* p;
   long long batch, row, head;
 };
-// 32 columns from c0 on of a row, of which those in front of head_dim exist
+// 16 columns from c0 on of a row, of which those in front of head_dim exist.  rest (its row, or null) gets what the
+// rounding took: out + rest is right to 2^-16, which D is taken from.  (From out alone D carries a rounding
+// of |do||o|, and the scores' gradient half as much error again.)
 template <typename T>
-__device__ __forceinline__ void store_row(const OutTensor& o, int b, int t, int h, int c0, int head_dim,
-                                          const uint32_t* v, float factor) {
+__device__ __forceinline__ void store16_of(const OutTensor& o, int b, int t, int h, int c0, int head_dim,
+                                           const uint32_t* v, float factor, T* rest) {
   T* to = static_cast<T*>(o.p) + b * o.batch + t * o.row + h * o.head + c0;
-  const auto two = [&](int e) {
-    return pack2<T>(__uint_as_float(v[e]) * factor, __uint_as_float(v[e + 1]) * factor);
-  };
 #pragma unroll
-  for (int u = 0; u < 4; ++u)
-    if (c0 + 8 * u < head_dim)
-      *reinterpret_cast<uint4*>(to + 8 * u) = make_uint4(two(8 * u), two(8 * u + 2), two(8 * u + 4), two(8 * u + 6));
+  for (int u = 0; u < 16; u += 8)
+    if (c0 + u < head_dim) {
+      float x[8], y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(v[u + e]) * factor;
+      const Vec16<T> r = pack16<T>(x);
+      store16(to + u, r);
+      if (rest) {
+        unpack16(r, y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = x[e] - y[e];
+        store16(rest + c0 + u, pack16<T>(y));
+      }
+    }
 }
 
 struct AttnShape {
@@ -324,26 +338,31 @@ struct AttnShape {
 };
 
 // ------------------------------------------------------------------------------------------ forward
-// One CTA takes 256 queries of a head, as two tiles with four warps each (a thread per row); the tiles
-// share the keys' blocks, and while one tile's warps are at its softmax the tensor pipe is at the other's products:
-//     S_t = Q_t K_j^T    columns 128 t ..         P_t over the same columns, 16 bits, the A operand of
-//     O_t += P_t V_j     columns 256 + D t ..     (kept over j)
-// P is exp2 of the scores less a reference that is raised, and O rescaled, only where a row's maximum passed
-// it by more than 2^8: rarely behind the first blocks.  P up to 2^8 loses nothing in either type.
+// One CTA takes 128 queries of a head and walks the keys' blocks, two CTAs to an SM: while one is at its softmax the
+// tensor pipe is at the other's products.
+//     S = Q K_j^T    columns 0 ..       P over the same columns, 16 bits, the A operand of
+//     O += P V_j     columns 128 ..     (kept over j)
+// Two threads share a row, half of the columns each, and agree on its maximum through shared memory.  P is exp2 of
+// the scores less a reference that is raised, and O rescaled, only where a row's maximum passed it by more than
+// 2^8: rarely behind the first blocks.  P up to 2^8 loses nothing in either type.
+// Sixteen warps of softmax on an SM, for each scheduler four, hide each other's waits for tensor memory and
+// exponentials; eight (a thread per row) left it idle half the time.
 template <int D>
 struct FwdSmem {
-  static constexpr int kTile = D / 64 * kBox, kStages = D == 64 ? 3 : 2;
-  static constexpr int kTotal = 2 * kTile + 2 * kStages * kTile + 1024 + 256;
+  static constexpr int kTile = D / 64 * kBox, kStages = D == 64 ? 2 : 1;
+  static constexpr int kExchange = 2 * 2 * 128 * 4;  // two buffers of a float per row and half
+  static constexpr int kTotal = kTile + 2 * kStages * kTile + kExchange + 1024 + 256;
+  static_assert(2 * kTotal <= 227 * 1024, "two CTAs to an SM");
 };
 struct AttnFwdArgs {
   AttnShape s;
   OutTensor out;
+  void* rest;  // [batch][q_len][heads][head_dim]: what out's rounding took, or null
   float* lse;  // [batch][heads][q_len], or null
-  int pairs;
 };
 
 template <int D, typename T, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(kThreads2, 1)
+__global__ void __maxnreg__(96)
 masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v, const AttnFwdArgs a) {
   chain_begin();
@@ -351,34 +370,21 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   constexpr int kStages = SM::kStages, kTile = SM::kTile;
   extern __shared__ __align__(1024) char smem_raw[];
   char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  char *sQ = base, *sK = base + 2 * kTile, *sV = sK + kStages * kTile;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + kStages * kTile);
+  char *sQ = base, *sK = base + kTile, *sV = sK + kStages * kTile;
+  float* exchange = reinterpret_cast<float*>(sV + kStages * kTile);  // [2][2 halves][128 rows]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(exchange + 512);
   uint64_t *bar_q = bars, *k_full = bars + 1, *k_empty = k_full + kStages, *v_full = k_empty + kStages,
-           *v_empty = v_full + kStages, *bar_s = v_empty + kStages, *bar_p = bar_s + 2, *bar_o = bar_p + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_o + 2);
+           *v_empty = v_full + kStages, *bar_s = v_empty + kStages, *bar_p = bar_s + 1, *bar_o = bar_p + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_o + 1);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int pair = a.pairs - 1 - (int)blockIdx.x % a.pairs;  // the longest of a causal head first
-  const int bh = blockIdx.x / a.pairs, batch = bh / a.s.heads, head = bh - batch * a.s.heads;
   const int nq = blocks_of(a.s.q_len), off = a.s.k_len - a.s.q_len;
-
-  // the key blocks of the two tiles
-  int begin[2], end[2];
-  int4 info[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    info[t] = make_int4(0, 0, 0, 0);
-    if (2 * pair + t < nq) info[t] = a.s.mask.q_blocks[(long long)batch * nq + 2 * pair + t];
-    begin[t] = end[t] = 0;
-    if (info[t].y > info[t].x) {
-      begin[t] = info[t].x / kBlock;
-      end[t] = blocks_of(info[t].y);
-    }
-  }
-  const bool both = end[0] > begin[0] && end[1] > begin[1];
-  const int j0 = both ? min(begin[0], begin[1]) : (end[0] > begin[0] ? begin[0] : begin[1]);
-  const int j1 = max(end[0], end[1]);  // (j1 = j0 = 0 where neither sees anything)
+  const int i = nq - 1 - (int)blockIdx.x % nq;  // the longest of a causal head first
+  const int bh = blockIdx.x / nq, batch = bh / a.s.heads, head = bh - batch * a.s.heads;
+  const int4 info = a.s.mask.q_blocks[(long long)batch * nq + i];
+  const int begin = info.y > info.x ? info.x / kBlock : 0;
+  const int blocks = info.y > info.x ? blocks_of(info.y) - begin : 0;
 
   if (threadIdx.x == 0) {
     mbar_init(bar_q, 1);
@@ -388,15 +394,13 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
     }
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(&bar_s[t], 1);
-      mbar_init(&bar_p[t], 4);
-      mbar_init(&bar_o[t], 1);
-    }
+    mbar_init(bar_s, 1);
+    mbar_init(bar_p, 8);
+    mbar_init(bar_o, 1);
     *failed = 0;
     fence_barrier_init();
   }
-  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  if (warp == 9) tmem_alloc(tmem_slot, 256);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -407,14 +411,12 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   };
 
   if (warp == 8) {
-    if (j1 > j0 && elect_one()) {
-      const int tiles = 2 * pair + 1 < nq ? 2 : 1;
-      mbar_expect_tx(bar_q, tiles * kTile);
-      for (int t = 0; t < tiles; ++t)
-        load_tile<D>(&map_q, bar_q, sQ + t * kTile, (2 * pair + t) * kBlock, head, batch);
+    if (blocks > 0 && elect_one()) {
+      mbar_expect_tx(bar_q, kTile);
+      load_tile<D>(&map_q, bar_q, sQ, i * kBlock, head, batch);
       const int kv = head / a.s.group;
       uint32_t s = 0, round = 0;
-      for (int j = j0; j < j1; ++j) {
+      for (int j = begin; j < begin + blocks; ++j) {
         if (round > 0) wait(&k_empty[s], (round - 1) & 1, 1);
         mbar_expect_tx(&k_full[s], kTile);
         load_tile<D>(&map_k, &k_full[s], sK + s * kTile, j * kBlock, kv, batch);
@@ -425,178 +427,173 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       }
     }
   } else if (warp == 9) {
-    if (j1 > j0 && elect_one()) {
+    if (blocks > 0 && elect_one()) {
       constexpr int kOperand = std::is_same<T, __half>::value ? kOperandF16 : kOperandBf16;
       const uint32_t id_s = umma_idesc_f16(kOperand, kBlock, 0, 0), id_o = umma_idesc_f16(kOperand, D, 0, 1);
       const uint64_t dQ = k_major<D>(sQ), dK = k_major<D>(sK), dV = mn_major<D>(sV);
-      auto active = [&](int t, int j) { return j >= begin[t] && j < end[t]; };
-      auto scores = [&](int t, uint32_t s) {
+      uint32_t ks = 0, k_round = 0, vs = 0, v_round = 0;
+      auto scores = [&] {
+        wait(&k_full[ks], k_round & 1, 4);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma_f16(tmem + 128 * t, umma_desc_advance(dQ, t * kTile + k_step(kk)),
-                   umma_desc_advance(dK, s * kTile + k_step(kk)), id_s, kk > 0);
-        umma_commit(&bar_s[t]);
+          umma_f16(tmem, umma_desc_advance(dQ, k_step(kk)), umma_desc_advance(dK, ks * kTile + k_step(kk)), id_s,
+                   kk > 0);
+        umma_commit(bar_s);
+        umma_commit(&k_empty[ks]);
+        if (++ks == kStages) { ks = 0; ++k_round; }
       };
-      uint32_t done[2] = {0, 0};  // blocks of each tile
-      uint32_t ks = 0, k_round = 0, vs = 0, v_round = 0;
       wait(bar_q, 0, 3);
-      wait(&k_full[0], 0, 4);
-      for (int t = 0; t < 2; ++t)
-        if (active(t, j0)) scores(t, 0);
-      umma_commit(&k_empty[0]);
-      if (++ks == kStages) { ks = 0; ++k_round; }
-      for (int j = j0; j < j1; ++j) {
-        bool next_here = false;
-        for (int t = 0; t < 2; ++t) {
-          if (active(t, j)) {
-            wait(&bar_p[t], done[t] & 1, 5);
-            wait(&v_full[vs], v_round & 1, 6);
+      scores();
+      for (int it = 0; it < blocks; ++it) {
+        wait(&v_full[vs], v_round & 1, 6);
+        wait(bar_p, it & 1, 5);
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk)  // K = 128 keys
-              umma_f16_ts(tmem + 256 + D * t, tmem + 128 * t + 8 * kk,
-                          umma_desc_advance(dV, vs * kTile + kk * 2048), id_o, (done[t] > 0 || kk > 0) ? 1u : 0u);
-            umma_commit(&bar_o[t]);
-            ++done[t];
-          }
-          if (j + 1 < j1 && active(t, j + 1)) {
-            if (!next_here) wait(&k_full[ks], k_round & 1, 7);
-            next_here = true;
-            scores(t, ks);
-          }
-        }
-        // (a block that neither tile meets is loaded all the same, and handed back)
-        if (!active(0, j) && !active(1, j)) wait(&v_full[vs], v_round & 1, 6);
+        for (int kk = 0; kk < 8; ++kk)  // K = 128 keys
+          umma_f16_ts(tmem + 128, tmem + 8 * kk, umma_desc_advance(dV, vs * kTile + kk * 2048), id_o,
+                      (it > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(bar_o);
         umma_commit(&v_empty[vs]);
         if (++vs == kStages) { vs = 0; ++v_round; }
-        if (j + 1 < j1) {
-          if (!next_here) wait(&k_full[ks], k_round & 1, 7);
-          umma_commit(&k_empty[ks]);
-          if (++ks == kStages) { ks = 0; ++k_round; }
-        }
+        if (it + 1 < blocks) scores();  // (behind the product that reads P, in the pipe's order)
       }
     }
   } else {
-    const int t = warp >> 2;
-    const int row = (warp & 3) * 32 + lane;
-    const int q = (2 * pair + t) * kBlock + row;
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const int q = i * kBlock + row;
     const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t s_addr = lane_addr + 128u * t, o_addr = lane_addr + 256u + (uint32_t)(D * t);
+    const uint32_t s_addr = lane_addr + 64u * half, p_addr = lane_addr + 32u * half;
+    const uint32_t o_addr = lane_addr + 128u + (uint32_t)(D / 2 * half);
     int2 seen = make_int2(0, 0);
     if (q < a.s.q_len) seen = a.s.mask.rows[(long long)batch * a.s.q_len + q];
     const float slope = BIAS ? a.s.slopes[head] * kLog2e : 0.f;
-    const float pos = (float)(q + off);
     float ref = -1e30f, sum = 0.f;  // in powers of 2; a row that has seen nothing yet is far below all scores
-    const int blocks = end[t] - begin[t];
     for (int it = 0; it < blocks; ++it) {
-      const int key0 = (begin[t] + it) * kBlock;
-      uint32_t raw[4][32];
-      wait(&bar_s[t], it & 1, 8);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) ld32_begin(s_addr + 32 * c, raw[c]);
+      const int key0 = (begin + it) * kBlock + 64 * half;  // this thread's 64 keys
+      uint32_t s[2][32];
+      wait(bar_s, it & 1, 8);
+      ld32_begin(s_addr, s[0]);
+      ld32_begin(s_addr + 32, s[1]);
       wait_ld();
-#pragma unroll
-      for (int c = 0; c < 4; ++c) settle(raw[c]);
-      float s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int e = 0; e < 32; ++e) s[c][e] = __uint_as_float(raw[c][e]);
-      // The scores in powers of 2.  (Without cap and bias they stay as they are, the factor is positive and comes
+      settle(s[0]);
+      settle(s[1]);
+      // The scores in powers of 2.  (Without cap and bias they stay as they are: the factor is positive and comes
       // with the subtraction below.)
       if constexpr (CAP || BIAS) {
+        const float apart = (float)(q + off - key0);
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            float z = CAP ? fmaf(-2.f * a.s.cap_log2, rcp(1.f + ex2(s[c][e] * a.s.to_2u_log2)), a.s.cap_log2)
-                          : s[c][e] * a.s.to_log2;
-            if (BIAS) z = fmaf(-slope, fabsf(pos - (float)(key0 + 32 * c + e)), z);
-            s[c][e] = z;
+          for (int e = 0; e < 32; e += 2) {
+            F2 z = pair(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+            if (CAP) {
+              float z0, z1;
+              unpair(z * pair(a.s.to_2u_log2), z0, z1);
+              z = fused(pair(rcp(1.f + ex2(z0)), rcp(1.f + ex2(z1))), pair(-2.f * a.s.cap_log2), pair(a.s.cap_log2));
+            } else {
+              z = z * pair(a.s.to_log2);
+            }
+            if (BIAS)
+              z = fused(pair(fabsf(apart - (float)(32 * c + e)), fabsf(apart - (float)(32 * c + e + 1))), pair(-slope),
+                        z);
+            float z0, z1;
+            unpair(z, z0, z1);
+            s[c][e] = __float_as_uint(z0);
+            s[c][e + 1] = __float_as_uint(z1);
           }
       }
       // (blocks that all rows see whole need no test per element)
-      if (!(info[t].z <= key0 && info[t].w >= key0 + kBlock)) {
+      if (!(info.z <= key0 && info.w >= key0 + 64)) {
         const unsigned width = (unsigned)max(seen.y - seen.x, 0);
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if ((unsigned)(key0 + 32 * c + e - seen.x) >= width) s[c][e] = -INFINITY;
+            if ((unsigned)(key0 + 32 * c + e - seen.x) >= width) s[c][e] = 0xff800000u;  // -infinity
       }
       float mx4[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        mx4[c] = s[c][0];
+        mx4[c] = __uint_as_float(s[c >> 1][16 * (c & 1)]);
 #pragma unroll
-        for (int e = 1; e < 32; ++e) mx4[c] = fmaxf(mx4[c], s[c][e]);
+        for (int e = 1; e < 16; ++e) mx4[c] = fmaxf(mx4[c], __uint_as_float(s[c >> 1][16 * (c & 1) + e]));
       }
       float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       if constexpr (!CAP && !BIAS) mx *= a.s.to_log2;
+      float* met = exchange + (it & 1) * 256 + row;
+      met[128 * half] = mx;
+      // the two warps that share these rows; behind it P may lie over the scores, which both have read
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+      mx = fmaxf(mx, met[128 * (half ^ 1)]);
       const bool raise = mx > ref + 8.f;
       if (__any_sync(0xffffffffu, raise)) {
         const float next = raise ? mx : ref, alpha = raise ? ex2(ref - next) : 1.f;
         ref = next;
         sum *= alpha;
         if (it > 0) {
-          wait(&bar_o[t], (it - 1) & 1, 9);
-#pragma unroll
-          for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            ld32_begin(o_addr + c, o);
+          wait(bar_o, (it - 1) & 1, 9);
+#pragma unroll 1
+          for (int c = 0; c < D / 2; c += 16) {
+            uint32_t o[16];
+            ld16_begin(o_addr + c, o);
             wait_ld();
-            settle(o);
+            settle16(o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            st32(o_addr + c, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            st16(o_addr + c, o);
           }
         }
       }
-      float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+      F2 sum2 = pair(0.f);
 #pragma unroll
-      for (int c = 0; c < 4; c += 2) {
-        uint32_t p[32];
+      for (int c = 0; c < 2; ++c) {
+        uint32_t p[16];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float p0, p1;
-            if constexpr (CAP || BIAS) {
-              p0 = ex2(s[c + h][e] - ref);
-              p1 = ex2(s[c + h][e + 1] - ref);
-            } else {
-              p0 = ex2(fmaf(s[c + h][e], a.s.to_log2, -ref));
-              p1 = ex2(fmaf(s[c + h][e + 1], a.s.to_log2, -ref));
-            }
-            sum4[(e >> 1) & 3] += p0 + p1;
-            p[16 * h + e / 2] = pack2<T>(p0, p1);
-          }
-        st32(s_addr + 16 * c, p);
+        for (int e = 0; e < 32; e += 2) {
+          F2 z = pair(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+          if constexpr (CAP || BIAS) z = z + pair(-ref);
+          else z = fused(z, pair(a.s.to_log2), pair(-ref));
+          float p0, p1;
+          unpair(z, p0, p1);
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+          sum2 = sum2 + pair(p0, p1);
+          p[e / 2] = pack2<T>(p0, p1);
+        }
+        st16(p_addr + 16 * c, p);
       }
-      sum += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+      float s0, s1;
+      unpair(sum2, s0, s1);
+      sum += s0 + s1;
       wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive(&bar_p[t]);
+      if (lane == 0) arrive(bar_p);
     }
-    if (blocks > 0) wait(&bar_o[t], (blocks - 1) & 1, 10);
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    // (the exchange's other buffer was last read before the last block's barrier)
+    float* met = exchange + (blocks & 1) * 256 + row;
+    met[128 * half] = sum;
+    asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+    sum = half == 0 ? sum + met[128] : met[0] + sum;
+    if (blocks > 0) wait(bar_o, (blocks - 1) & 1, 10);
+    const float inv = sum > 0.f ? 1.f / sum : sum;  // (a sum that is not a number shows in the output)
+    const long long rest_at = (((long long)batch * a.s.q_len + q) * a.s.heads + head) * a.s.head_dim;
 #pragma unroll 1
-    for (int c = 0; c < D; c += 32) {
-      uint32_t o[32];
+    for (int c = 0; c < D / 2; c += 16) {
+      uint32_t o[16];
       __syncwarp();  // the lanes past the end store nothing, and are back for the next load
       if (blocks > 0) {
-        ld32_begin(o_addr + c, o);
+        ld16_begin(o_addr + c, o);
         wait_ld();
-        settle(o);
+        settle16(o);
       } else {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = 0;
+        for (int e = 0; e < 16; ++e) o[e] = 0;
       }
       if (q < a.s.q_len)
-        store_row<T>(a.out, batch, q, head, c, a.s.head_dim, o, inv);
+        store16_of<T>(a.out, batch, q, head, D / 2 * half + c, a.s.head_dim, o, inv,
+                      a.rest ? static_cast<T*>(a.rest) + rest_at : nullptr);
     }
-    // NaN among the scores shows in both
-    if (q < a.s.q_len && a.lse)
+    if (half == 0 && q < a.s.q_len && a.lse)
       a.lse[(long long)bh * a.s.q_len + q] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
   }
   if (*failed)  // copies and contractions under way when a wait ran out have ended after this
@@ -607,7 +604,7 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   if (threadIdx.x == 0 && *failed != 0 && a.s.status) atomicExch(a.s.status, *failed);
   if (warp == 9) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, 256);
   }
 }
 
@@ -892,19 +889,19 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
     const float factor = KV && h == 0 ? 1.f : a.s.scale;
     const int rows = KV ? a.s.k_len : a.s.q_len;
 #pragma unroll 1
-    for (int c = c_first; c < c_last; c += 32) {
-      uint32_t o[32];
+    for (int c = c_first; c < c_last; c += 16) {
+      uint32_t o[16];
       __syncwarp();
       if (total > 0) {
-        ld32_begin(from + c, o);
+        ld16_begin(from + c, o);
         wait_ld();
-        settle(o);
+        settle16(o);
       } else {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = 0;
+        for (int e = 0; e < 16; ++e) o[e] = 0;
       }
       if (mine < rows)
-        store_row<T>(out, batch, mine, head, c, a.s.head_dim, o, factor);
+        store16_of<T>(out, batch, mine, head, c, a.s.head_dim, o, factor, nullptr);
     }
   }
   if (*failed)
@@ -931,11 +928,11 @@ masked_backward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     backward_body<D, T, CAP, BIAS, false>(map_q, map_k, map_v, map_do, a, blockIdx.x - a.kv_ctas);
 }
 
-// D = rowsum(dO * O): sixteen lanes per row, one 16-byte load each.  Results in [batch][heads][q_len].
+// D = rowsum(dO * (O + rest)): sixteen lanes per row, one 16-byte load each.  Results in [batch][heads][q_len].
 template <typename T>
 __global__ void __launch_bounds__(256)
-masked_dsum_kernel(const OutTensor o, const OutTensor go, float* __restrict__ dsum, long long rows, int q_len,
-                   int heads, int head_dim) {
+masked_dsum_kernel(const OutTensor o, const T* __restrict__ rest, const OutTensor go, float* __restrict__ dsum,
+                   long long rows, int q_len, int heads, int head_dim) {
   chain_begin();
   const long long t = blockIdx.x * 256LL + threadIdx.x, r = t >> 4;
   const int c = 8 * (int)(t & 15);
@@ -951,6 +948,12 @@ masked_dsum_kernel(const OutTensor o, const OutTensor go, float* __restrict__ ds
       float x[8], g[8];
       unpack16(load16(static_cast<const T*>(o.p) + b * o.batch + i * o.row + h * o.head + c), x);
       unpack16(load16(static_cast<const T*>(go.p) + b * go.batch + i * go.row + h * go.head + c), g);
+      if (rest) {
+        float y[8];
+        unpack16(load16(rest + r * head_dim + c), y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] += y[e];
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) acc = fmaf(x[e], g[e], acc);
     }
@@ -1023,8 +1026,7 @@ int launch_forward(const flb200_attention_desc* d, const CUtensorMap& mq, const 
                    AttnFwdArgs a, cudaStream_t st) {
   const auto kernel = masked_forward_kernel<D, T, CAP, BIAS>;
   if (int rc = configure(reinterpret_cast<const void*>(kernel), FwdSmem<D>::kTotal)) return rc;
-  a.pairs = (blocks_of(d->q_len) + 1) / 2;
-  launch_chained(kernel, (unsigned)(d->batch * d->heads * a.pairs), kThreads2, FwdSmem<D>::kTotal, st, mq, mk, mv, a);
+  launch_chained(kernel, (unsigned)(d->batch * d->heads * blocks_of(d->q_len)), kThreads2, FwdSmem<D>::kTotal, st, mq, mk, mv, a);
   FLB200_AFTER_LAUNCH("masked_attention_forward");
   count_tc_launch();
   return FLB200_OK;
@@ -1091,9 +1093,11 @@ int flb200_masked_attention_supported(const flb200_attention_desc* d) {
 
 int flb200_masked_attention_forward(const flb200_attention_desc* d, const flb200_head_tensor* q,
                                     const flb200_head_tensor* k, const flb200_head_tensor* v, const float* slopes,
-                                    const void* mask, const flb200_head_tensor* out, float* lse, void* stream) {
+                                    const void* mask, const flb200_head_tensor* out, void* rest, float* lse,
+                                    void* stream) {
   if (int rc = check_attention("masked_attention_forward", d)) return rc;
   FLB200_REQUIRE(mask, "masked_attention_forward: null mask");
+  FLB200_REQUIRE(!rest || aligned16(rest), "masked_attention_forward: rest must be 16-byte aligned");
   for (const flb200_head_tensor* t : {q, k, v, out})
     if (int rc = check_tensor("masked_attention_forward", t)) return rc;
   const int operand = operand_of(d->dtype);
@@ -1104,6 +1108,7 @@ int flb200_masked_attention_forward(const flb200_attention_desc* d, const flb200
   AttnFwdArgs a{};
   a.s = shape_of(d, slopes, mask);
   a.out = out_of(*out);
+  a.rest = rest;
   a.lse = lse;
   return dispatch(d, slopes != nullptr, [&](auto dim, auto type, auto cap, auto bias) {
     return launch_forward<decltype(dim)::value, decltype(type), decltype(cap)::value, decltype(bias)::value>(
@@ -1118,13 +1123,14 @@ size_t flb200_masked_attention_backward_workspace_bytes(const flb200_attention_d
 
 int flb200_masked_attention_backward(const flb200_attention_desc* d, const flb200_head_tensor* q,
                                      const flb200_head_tensor* k, const flb200_head_tensor* v,
-                                     const flb200_head_tensor* out, const flb200_head_tensor* grad_out,
-                                     const float* lse, const float* slopes, const void* mask,
+                                     const flb200_head_tensor* out, const void* rest,
+                                     const flb200_head_tensor* grad_out, const float* lse, const float* slopes, const void* mask,
                                      const flb200_head_tensor* grad_q, const flb200_head_tensor* grad_k,
                                      const flb200_head_tensor* grad_v, void* workspace, size_t workspace_bytes,
                                      void* stream) {
   if (int rc = check_attention("masked_attention_backward", d)) return rc;
   FLB200_REQUIRE(mask && lse, "masked_attention_backward: null mask or lse");
+  FLB200_REQUIRE(!rest || aligned16(rest), "masked_attention_backward: rest must be 16-byte aligned");
   for (const flb200_head_tensor* t : {q, k, v, out, grad_out, grad_q, grad_k, grad_v})
     if (int rc = check_tensor("masked_attention_backward", t)) return rc;
   const size_t need = flb200_masked_attention_backward_workspace_bytes(d);
@@ -1141,11 +1147,13 @@ int flb200_masked_attention_backward(const flb200_attention_desc* d, const flb20
   const long long rows = d->batch * d->heads * d->q_len;
   const unsigned grid = (unsigned)((rows * 16 + 255) / 256);
   if (d->dtype == FLB200_F16)
-    launch_chained(masked_dsum_kernel<__half>, grid, 256, 0, st, out_of(*out), out_of(*grad_out), dsum, rows,
-                   (int)d->q_len, (int)d->heads, (int)d->head_dim);
+    launch_chained(masked_dsum_kernel<__half>, grid, 256, 0, st, out_of(*out),
+                   static_cast<const __half*>(rest), out_of(*grad_out), dsum, rows, (int)d->q_len, (int)d->heads,
+                   (int)d->head_dim);
   else
-    launch_chained(masked_dsum_kernel<__nv_bfloat16>, grid, 256, 0, st, out_of(*out), out_of(*grad_out), dsum, rows,
-                   (int)d->q_len, (int)d->heads, (int)d->head_dim);
+    launch_chained(masked_dsum_kernel<__nv_bfloat16>, grid, 256, 0, st, out_of(*out),
+                   static_cast<const __nv_bfloat16*>(rest), out_of(*grad_out), dsum, rows, (int)d->q_len, (int)d->heads,
+                   (int)d->head_dim);
   FLB200_AFTER_LAUNCH("masked_attention_dsum");
   AttnBwdArgs a{};
   a.s = shape_of(d, slopes, mask);

@@ -707,33 +707,40 @@ struct AttentionCall {
     }
   }
 };
-NATIVE(masked_attention) {  // (AttentionCall's) -> (out, lse)
+NATIVE(masked_attention) {  // (AttentionCall's, train) -> (out, lse, rest), the last two None unless train
   AttentionCall c(x);
   const flb200_attention_desc& d = c.d;
   const Tensor& q = x.tensor(0);
-  Tensor out = empty({d.batch, d.q_len, d.heads, d.head_dim}, q.scalar_type(), q);
-  Tensor lse = empty({d.batch, d.heads, d.q_len}, ScalarType::Float, q);
+  Tensor out = empty({d.batch, d.q_len, d.heads, d.head_dim}, q.scalar_type(), q), lse, rest;
+  if (x.b(10)) {
+    lse = empty({d.batch, d.heads, d.q_len}, ScalarType::Float, q);
+    rest = empty_like(out);
+  }
   const Heads o(out, "out");
   check(unlocked(flb200_masked_attention_forward, &d, (const flb200_head_tensor*)&c.q.h,
-                 (const flb200_head_tensor*)&c.k.h, (const flb200_head_tensor*)&c.v.h, c.slopes, c.mask, &o.h, Pf(&lse),
-                 stream()));
-  return wrap({out, lse});
+                 (const flb200_head_tensor*)&c.k.h, (const flb200_head_tensor*)&c.v.h, c.slopes, c.mask, &o.h,
+                 rest.defined() ? P(rest) : nullptr, lse.defined() ? Pf(&lse) : nullptr, stream()));
+  return wrap({out, lse, rest});
 }
-// (AttentionCall's, out, grad_out, lse, grad_q, grad_k, grad_v or None three times: new tensors) -> (grad_q, ...)
+// (AttentionCall's, out, rest, grad_out, lse, grad_q, grad_k, grad_v or None three times: new tensors)
+//   -> (grad_q, grad_k, grad_v)
 NATIVE(masked_attention_backward) {
   AttentionCall c(x);
   const flb200_attention_desc& d = c.d;
-  const Tensor &out = x.tensor(10), &gy = x.tensor(11), &lse = x.tensor(12);
+  const Tensor &out = x.tensor(10), &gy = x.tensor(12), &lse = x.tensor(13);
+  const Tensor* rest = x.t(11);
   if (out.sizes() != x.tensor(0).sizes() || gy.sizes() != out.sizes() || gy.scalar_type() != out.scalar_type() ||
       out.scalar_type() != x.tensor(0).scalar_type())
     value_error("masked_attention: the output's gradient must be like the output");
   if (lse.numel() != d.batch * d.heads * d.q_len || lse.scalar_type() != ScalarType::Float)
     value_error("masked_attention: lse does not belong to these tensors");
+  if (rest && (rest->numel() != out.numel() || rest->scalar_type() != out.scalar_type() || !rest->is_contiguous()))
+    value_error("masked_attention: rest does not belong to these tensors");
   const Heads o(out, "out"), g(gy, "grad_out");
   Tensor grads[3];
   for (int i = 0; i < 3; ++i) {
     const Tensor& like = x.tensor(i);
-    const Tensor* given = x.t(13 + i);
+    const Tensor* given = x.t(14 + i);
     if (given && (given->sizes() != like.sizes() || given->scalar_type() != like.scalar_type() || !Heads::fits(*given)))
       value_error("masked_attention: a given gradient must be like its tensor, in aligned rows");
     grads[i] = given ? *given : empty(like.sizes(), like.scalar_type(), like);
@@ -741,7 +748,7 @@ NATIVE(masked_attention_backward) {
   const Heads gq(grads[0], "grad_q"), gk(grads[1], "grad_k"), gv(grads[2], "grad_v");
   Workspace ws(flb200_masked_attention_backward_workspace_bytes(&d), out);
   check(unlocked(flb200_masked_attention_backward, &d, (const flb200_head_tensor*)&c.q.h,
-                 (const flb200_head_tensor*)&c.k.h, (const flb200_head_tensor*)&c.v.h, &o.h, &g.h,
+                 (const flb200_head_tensor*)&c.k.h, (const flb200_head_tensor*)&c.v.h, &o.h, (const void*)P(rest), &g.h,
                  (const float*)Pf(&lse), c.slopes, c.mask, &gq.h, &gk.h, &gv.h, ws.p(), ws.bytes, stream()));
   return wrap({grads[0], grads[1], grads[2]});
 }

@@ -351,15 +351,17 @@ def attention_mask(batch: int, q_len: int, k_len: Optional[int] = None, *, causa
     return AttentionMask(batch, q_len, k_len, N.attention_mask(batch, q_len, k_len, causal, documents, prefix, index))
 
 
-def masked_attention(q, k, v, mask: AttentionMask, scale: float, softcap: float = 0.0, slopes=None):
+def masked_attention(q, k, v, mask: AttentionMask, scale: float, softcap: float = 0.0, slopes=None,
+                     train: bool = True):
     """softmax(softcap * tanh(scale q k^T / softcap) - slopes |i - j|) v over the keys that the mask leaves, in one
     kernel: q (batch, q_len, heads, head dim), k and v (batch, k_len, key heads, head dim), f16 or bf16, any strides
-    (those of whole 16-byte rows are read in place).  slopes: float32 per query head, or None.  Returns (out, lse)."""
-    return N.masked_attention(q, k, v, slopes, mask.data, mask.batch, mask.q_len, mask.k_len, scale, softcap)
+    (those of whole 16-byte rows are read in place).  slopes: float32 per query head, or None.  Returns (out, lse,
+    rest): what the gradient needs besides, each row's log-sum-exp and what the rounding of out took, or None."""
+    return N.masked_attention(q, k, v, slopes, mask.data, mask.batch, mask.q_len, mask.k_len, scale, softcap, train)
 
 
-def masked_attention_backward(q, k, v, out, grad_out, lse, mask: AttentionMask, scale: float, softcap: float = 0.0,
-                              slopes=None, grads=(None, None, None)):
+def masked_attention_backward(q, k, v, out, rest, grad_out, lse, mask: AttentionMask, scale: float,
+                              softcap: float = 0.0, slopes=None, grads=(None, None, None)):
     """(grad_q, grad_k, grad_v) of masked_attention, into the tensors of `grads` where they are given."""
     return N.masked_attention_backward(q, k, v, slopes, mask.data, mask.batch, mask.q_len, mask.k_len, scale, softcap,
-                                       out, grad_out, lse, *grads)
+                                       out, rest, grad_out, lse, *grads)

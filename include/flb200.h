@@ -613,7 +613,9 @@ int flb200_attention_mask(int64_t batch, int64_t q_len, int64_t k_len, int causa
  * probabilities and the scores' gradient are rounded to the tensors' type as operands.  Tensors by strides in
  * elements, each a multiple of 8, data 16-byte aligned: element (b, t, h, d) at b*batch + t*row + h*head + d.
  * The values of k and v in a block of 128 positions that some query of a block sees must be finite, or that
- * query block's output is not.  lse: fp32 [batch][heads][q_len] (NULL in forward: not kept).
+ * query block's output is not.  For the gradient forward keeps lse, fp32 [batch][heads][q_len], and rest
+ * [batch][q_len][heads][head_dim], what the rounding of out took, in the tensors' type; either may be NULL, and
+ * without rest the gradient of the scores carries a rounding of out more.
  * Backward gives the gradients of q, k and v (those of k and v summed over the heads that share them), without
  * atomics: equal inputs give equal bits. */
 typedef struct flb200_attention_desc {
@@ -629,12 +631,12 @@ int flb200_masked_attention_supported(const flb200_attention_desc* d);
 int flb200_masked_attention_forward(const flb200_attention_desc* d, const flb200_head_tensor* q,
                                     const flb200_head_tensor* k, const flb200_head_tensor* v,
                                     const float* slopes, const void* mask, const flb200_head_tensor* out,
-                                    float* lse, void* stream);
+                                    void* rest, float* lse, void* stream);
 size_t flb200_masked_attention_backward_workspace_bytes(const flb200_attention_desc* d);
 int flb200_masked_attention_backward(const flb200_attention_desc* d, const flb200_head_tensor* q,
                                      const flb200_head_tensor* k, const flb200_head_tensor* v,
-                                     const flb200_head_tensor* out, const flb200_head_tensor* grad_out,
-                                     const float* lse, const float* slopes, const void* mask,
+                                     const flb200_head_tensor* out, const void* rest,
+                                     const flb200_head_tensor* grad_out, const float* lse, const float* slopes, const void* mask,
                                      const flb200_head_tensor* grad_q, const flb200_head_tensor* grad_k,
                                      const flb200_head_tensor* grad_v, void* workspace, size_t workspace_bytes,
                                      void* stream);

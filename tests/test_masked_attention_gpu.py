@@ -2,8 +2,8 @@
 
 Tolerances.  Scores, statistics and sums are fp32 (2^-21 and below).  P and dS are rounded once to the tensors' type
 before their products and the result once more: relative to a result's norm each rounding is at most u = 2^-9
-(bf16) or 2^-12 (f16) of the products' terms, which add up at random or better.  D takes the rounded output, another u
-of |do||o|.  4 u holds the four gradients and the output with room, tested on the norm per head; the lse to 2e-5."""
+(bf16) or 2^-12 (f16) of the products' terms, which add up at random or better.  4 u holds the gradients and the
+output with room, tested on the norm per head; the lse to 2e-5."""
 import math
 import random
 
@@ -195,8 +195,8 @@ def test_strides_and_packed(dtype):
         for a, b in zip(vs, same):
             assert torch.equal(a.grad, b.grad)
     one = parts[1][:1].expand(B, T, Hk, D)
-    o4, _ = F.masked_attention(parts[0], one, one, mask, 0.1)
-    o5, _ = F.masked_attention(parts[0], one.contiguous(), one.contiguous(), mask, 0.1)
+    o4 = F.masked_attention(parts[0], one, one, mask, 0.1)[0]
+    o5 = F.masked_attention(parts[0], one.contiguous(), one.contiguous(), mask, 0.1)[0]
     assert torch.equal(o4, o5)
 
 
@@ -223,7 +223,7 @@ def test_values_behind_the_mask():
     got = F.masked_attention(q, k2, v, mask, 0.125)[0]
     assert torch.equal(got[:, :100], clean[0][:, :100])
     # gradients of the rows that count, with the padding's dO infinite in the rows that do not exist for the mask
-    grads = F.masked_attention_backward(q, k, v, clean[0], go, clean[1], mask, 0.125)
+    grads = F.masked_attention_backward(q, k, v, clean[0], clean[2], go, clean[1], mask, 0.125)
     assert all(bool(torch.isfinite(x).all()) for x in grads)
     assert bool((grads[1][:, 256:] == 0).all()) and bool((grads[2][:, 256:] == 0).all())
     assert bool((grads[0][:, 256:] == 0).all())
@@ -240,10 +240,10 @@ def test_large_scores_and_equal_bits():
     seen = visible(B, T, T, True)
     want = definition(q, k, v, go, seen, 1.0, 0.0, None)
     mask = F.attention_mask(B, T)
-    out, lse = F.masked_attention(q, k, v, mask, 1.0)
+    out, lse, rest = F.masked_attention(q, k, v, mask, 1.0)
     near(out, want[0], UNIT[torch.bfloat16], "out")
-    a = F.masked_attention_backward(q, k, v, out, go, lse, mask, 1.0)
-    b = F.masked_attention_backward(q, k, v, out, go, lse, mask, 1.0)
+    a = F.masked_attention_backward(q, k, v, out, rest, go, lse, mask, 1.0)
+    b = F.masked_attention_backward(q, k, v, out, rest, go, lse, mask, 1.0)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
     for got, w, name in zip(a, want[2:], ("dq", "dk", "dv")):
         near(got, w, 4 * UNIT[torch.bfloat16], name)
@@ -256,8 +256,8 @@ def test_gradient_is_the_differences():
     q, k, v, go = (torch.randn(B, T, H, D, generator=g, device="cuda").half() for _ in range(4))
     mask = F.attention_mask(B, T)
     slopes = torch.tensor([0.1, 0.3], device="cuda")
-    out, lse = F.masked_attention(q, k, v, mask, 0.3, 4.0, slopes)
-    grads = F.masked_attention_backward(q, k, v, out, go, lse, mask, 0.3, 4.0, slopes)
+    out, lse, rest = F.masked_attention(q, k, v, mask, 0.3, 4.0, slopes)
+    grads = F.masked_attention_backward(q, k, v, out, rest, go, lse, mask, 0.3, 4.0, slopes)
     f = lambda a, b, c: float((F.masked_attention(a, b, c, mask, 0.3, 4.0, slopes)[0].double() * go.double()).sum())  # noqa: E731
     for i in range(3):
         e = torch.sign(grads[i].float()) * 2.0 ** -6
