@@ -35,7 +35,7 @@ using namespace tc;
 constexpr int kBlock = 128;        // queries and keys of a block
 constexpr int kBox = 128 * 128;    // bytes of [128 rows][64 16-bit values], one TMA box
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kThreads2 = 320;     // warps 0..7: two threads per row; 8: TMA; 9: MMA
+constexpr int kFwdThreads = 320;   // warps 0..7: two threads per row; 8: TMA; 9: MMA
 
 // ------------------------------------------------------------------------------------------ the mask
 // rows: [lo, hi) of each query ([batch][q_len]; hi <= lo: it sees nothing).  q_blocks: of each block of queries the
@@ -610,18 +610,23 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 
 // ------------------------------------------------------------------------------------------ gradient
 // Two kinds of CTA in one launch, alike but for what their rows are.  A tile of 128 rows stays in shared memory, the
-// other side comes by in blocks of 128 columns, as two halves with four warps each (a thread per row):
+// other side comes by in blocks of 128 columns, in units of 64, each unit some four warps' (a thread per row):
 //     dK, dV   rows = keys K_j V_j     columns = queries Q_i dO_i of all heads that share the key head
 //     dQ       rows = queries Q_i dO_i columns = keys K_j V_j
-//     S = rows1 cols1^T, dP = rows2 cols2^T     (128 x 64 each, columns 128 half .. of tensor memory)
+//     S = rows1 cols1^T, dP = rows2 cols2^T     (128 x 64 each, columns 128 k .. of tensor memory)
 //     P and dS over the same columns, 16 bits, A operands of
-//     dV += P cols2, dK += dS cols1   or   dQ += dS cols1     (columns 256 ..)
+//     dV += P cols2, dK += dS cols1   or   dQ += dS cols1     (the last 2 D columns)
+// What bounds a unit is its chain from contraction to P and dS to contraction, so as many units are under way as tensor
+// memory holds: three at 64 dimensions, two at 128.
 // Nothing is added across CTAs: the result does not depend on their order.  The price is that S and dP are made
 // twice, 7 contractions where sums in device memory need 5; those would cost 4 bytes a value per key block.
 template <int D>
 struct BwdSmem {
-  static constexpr int kTile = D / 64 * kBox, kStages = 2;
-  static constexpr int kColumns = 2 * 128 * 16;  // two buffers of lse and D, and of the interval, per query column
+  static constexpr int kUnits = D == 64 ? 3 : 2;  // under way: four warps, and 128 columns of tensor memory, each
+  // (the unit that is issued behind the last of a block lies up to kUnits / 2 blocks further)
+  static constexpr int kTile = D / 64 * kBox, kStages = D == 64 ? 3 : 2;
+  static constexpr int kThreads = (4 * kUnits + 2) * 32, kTma = 4 * kUnits, kMma = kTma + 1;  // (the last two warps)
+  static constexpr int kColumns = kUnits * 2 * 64 * 16;  // two buffers of lse, D and interval per query column
   static constexpr int kTotal = 2 * kTile + 2 * kStages * kTile + kColumns + 1024 + 256;
 };
 struct AttnBwdArgs {
@@ -637,15 +642,16 @@ __device__ __forceinline__ void
 backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, const CUtensorMap& map_do,
               const AttnBwdArgs& a, int cta) {
   using SM = BwdSmem<D>;
-  constexpr int kStages = SM::kStages, kTile = SM::kTile;
+  constexpr int kStages = SM::kStages, kTile = SM::kTile, kUnits = SM::kUnits;
+  constexpr uint32_t kSums = 512 - 2 * D;  // first column of the sums
   extern __shared__ __align__(1024) char smem_raw[];
   char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   char *sR1 = base, *sR2 = base + kTile, *sC1 = base + 2 * kTile, *sC2 = sC1 + kStages * kTile;
-  float2* columns = reinterpret_cast<float2*>(sC2 + kStages * kTile);  // [2][128] lse, D
-  int2* intervals = reinterpret_cast<int2*>(columns + 256);            // [2][128]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(intervals + 256);
-  uint64_t *bar_r = bars, *full = bars + 1, *empty = full + kStages, *bar_s = empty + kStages, *bar_p = bar_s + 2,
-           *bar_a = bar_p + 2;
+  float2* columns = reinterpret_cast<float2*>(sC2 + kStages * kTile);      // [kUnits][2][64] lse, D
+  int2* intervals = reinterpret_cast<int2*>(columns + kUnits * 128);       // [kUnits][2][64]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(intervals + kUnits * 128);
+  uint64_t *bar_r = bars, *full = bars + 1, *empty = full + kStages, *bar_s = empty + kStages,
+           *bar_p = bar_s + kUnits, *bar_a = bar_p + kUnits;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_a + 1);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -674,15 +680,15 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int h = 0; h < 2; ++h) {
-      mbar_init(&bar_s[h], 1);
-      mbar_init(&bar_p[h], 4);
+    for (int w = 0; w < kUnits; ++w) {
+      mbar_init(&bar_s[w], 1);
+      mbar_init(&bar_p[w], 4);
     }
     mbar_init(bar_a, 1);
     *failed = 0;
     fence_barrier_init();
   }
-  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  if (warp == SM::kMma) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -692,7 +698,7 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
     tc_fence_after();
   };
 
-  if (warp == 8) {
+  if (warp == SM::kTma) {
     if (total > 0 && elect_one()) {
       mbar_expect_tx(bar_r, 2 * kTile);
       load_tile<D>(KV ? &map_k : &map_q, bar_r, sR1, block * kBlock, head, batch);
@@ -708,57 +714,55 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
         if (++in_head == count) { in_head = 0; ++h; }
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == SM::kMma) {
     if (total > 0 && elect_one()) {
       constexpr int kOperand = std::is_same<T, __half>::value ? kOperandF16 : kOperandBf16;
       const uint32_t id_s = umma_idesc_f16(kOperand, 64, 0, 0), id_a = umma_idesc_f16(kOperand, D, 0, 1);
       const uint64_t dR1 = k_major<D>(sR1), dR2 = k_major<D>(sR2), dC1 = k_major<D>(sC1), dC2 = k_major<D>(sC2);
       const uint64_t mC1 = mn_major<D>(sC1), mC2 = mn_major<D>(sC2);
-      auto scores = [&](int h, uint32_t s) {  // rows 64 h .. of the column tiles
-        const uint32_t at = s * kTile + h * 8192;
+      const int units = 2 * total;
+      uint32_t next_s = 0, next_round = 0;  // of the block whose scores come next
+      auto scores = [&](int u, int w) {     // rows 64 (u % 2) .. of its block's tiles
+        if ((u & 1) == 0) wait(&full[next_s], next_round & 1, 3);
+        const uint32_t at = next_s * kTile + (u & 1) * 8192;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma_f16(tmem + 128 * h, umma_desc_advance(dR1, k_step(kk)), umma_desc_advance(dC1, at + k_step(kk)), id_s,
+          umma_f16(tmem + 128 * w, umma_desc_advance(dR1, k_step(kk)), umma_desc_advance(dC1, at + k_step(kk)), id_s,
                    kk > 0);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma_f16(tmem + 128 * h + 64, umma_desc_advance(dR2, k_step(kk)), umma_desc_advance(dC2, at + k_step(kk)),
+          umma_f16(tmem + 128 * w + 64, umma_desc_advance(dR2, k_step(kk)), umma_desc_advance(dC2, at + k_step(kk)),
                    id_s, kk > 0);
-        umma_commit(&bar_s[h]);
+        umma_commit(&bar_s[w]);
+        if ((u & 1) && ++next_s == kStages) { next_s = 0; ++next_round; }
       };
-      uint32_t s = 0, round = 0;
       wait(bar_r, 0, 2);
-      wait(&full[0], 0, 3);
-      scores(0, 0);
-      scores(1, 0);
-      for (int it = 0; it < total; ++it) {
-        const uint32_t ns = s + 1 == kStages ? 0 : s + 1, nround = s + 1 == kStages ? round + 1 : round;
-        for (int h = 0; h < 2; ++h) {
-          wait(&bar_p[h], it & 1, 4);
+      for (int u = 0; u < kUnits && u < units; ++u) scores(u, u);
+      uint32_t s = 0;
+      int w = 0, k = 0;  // unit u is the k-th of its warps w
+      for (int u = 0; u < units; ++u) {
+        wait(&bar_p[w], k & 1, 4);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {  // K = 64 columns of this half
-            const uint32_t at = s * kTile + h * 8192 + kk * 2048, add = (it > 0 || h > 0 || kk > 0) ? 1u : 0u;
-            if (KV)
-              umma_f16_ts(tmem + 256, tmem + 128 * h + 8 * kk, umma_desc_advance(mC2, at), id_a, add);
-            umma_f16_ts(tmem + 256 + (KV ? D : 0), tmem + 128 * h + 64 + 8 * kk, umma_desc_advance(mC1, at), id_a, add);
-          }
-          if (h == 1) umma_commit(it + 1 < total ? &empty[s] : bar_a);
-          if (it + 1 < total) {
-            if (h == 0) wait(&full[ns], nround & 1, 3);
-            scores(h, ns);
-          }
+        for (int kk = 0; kk < 4; ++kk) {  // K = 64 columns
+          const uint32_t at = s * kTile + (u & 1) * 8192 + kk * 2048, add = (u > 0 || kk > 0) ? 1u : 0u;
+          if (KV) umma_f16_ts(tmem + kSums, tmem + 128 * w + 8 * kk, umma_desc_advance(mC2, at), id_a, add);
+          umma_f16_ts(tmem + kSums + D, tmem + 128 * w + 64 + 8 * kk, umma_desc_advance(mC1, at), id_a, add);
         }
-        s = ns;
-        round = nround;
+        if (u & 1) {
+          umma_commit(u + 1 < units ? &empty[s] : bar_a);
+          if (++s == kStages) s = 0;
+        }
+        if (u + kUnits < units) scores(u + kUnits, w);  // (behind the products that read P and dS, in the pipe's order)
+        if (++w == kUnits) { w = 0; ++k; }
       }
     }
   } else {
-    const int h = warp >> 2;                    // which half of the columns
+    const int w = warp >> 2;                    // of the units, every kUnits-th from w on
     const int row = (warp & 3) * 32 + lane;
     const int mine = block * kBlock + row;      // key or query
     const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t s_addr = lane_addr + 128u * h;
-    const int tid = threadIdx.x & 127;          // in the half's four warps
+    const uint32_t s_addr = lane_addr + 128u * w;
+    const int tid = threadIdx.x & 127;          // in the unit's four warps
     const long long rows0 = (long long)(KV ? batch * a.s.heads + head * a.s.group : bh) * a.s.q_len;
     // (a row that sees nothing, and what lies past the end: lse of infinity makes P zero)
     auto lse_of = [&](long long at) {
@@ -773,11 +777,11 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
       seen = a.s.mask.rows[(long long)batch * a.s.q_len + mine];
     }
     if (BIAS && !KV) slope = a.s.slopes[head] * kLog2e;
-    // of a query block's columns: lse, D and the interval, a thread per column
+    // of a unit's columns, where they are queries: lse, D and the interval, a thread per column
     struct Column { float2 ld; int2 seen; };
-    auto column = [&](int in_head, int hq) {
+    auto column = [&](int u, int in_head, int hq) {
       Column c{make_float2(INFINITY, 0.f), make_int2(0, 0)};
-      const int q = (first + in_head) * kBlock + 64 * h + tid;
+      const int q = (first + in_head) * kBlock + 64 * (u & 1) + tid;
       if (tid < 64 && q < a.s.q_len) {
         const long long at = rows0 + (long long)hq * a.s.q_len + q;
         c.seen = a.s.mask.rows[(long long)batch * a.s.q_len + q];
@@ -787,30 +791,36 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
     };
     auto keep = [&](int buffer, const Column& c) {
       if (tid < 64) {
-        columns[buffer * 128 + 64 * h + tid] = c.ld;
-        intervals[buffer * 128 + 64 * h + tid] = c.seen;
+        columns[(2 * w + buffer) * 64 + tid] = c.ld;
+        intervals[(2 * w + buffer) * 64 + tid] = c.seen;
       }
     };
-    if (KV && total > 0) keep(0, column(0, 0));
-    int in_head = 0, hq = 0;
-    for (int it = 0; it < total; ++it) {
-      const int col0 = (first + in_head) * kBlock + 64 * h;  // first column of this half
-      const float2* cols = columns + (it & 1) * 128 + 64 * h;
-      const int2* seen_by = intervals + (it & 1) * 128 + 64 * h;
+    // the block of unit u within its head, and the head
+    int in_head = w >> 1, hq = 0;
+    auto settle_head = [&] {
+      while (in_head >= count) { in_head -= count; ++hq; }
+    };
+    if (total > 0) settle_head();
+    if (KV && w < 2 * total) keep(0, column(w, in_head, hq));
+    for (int u = w, k = 0; u < 2 * total; u += kUnits, ++k) {
+      const int col0 = (first + in_head) * kBlock + 64 * (u & 1);
+      const float2* cols = columns + (2 * w + (k & 1)) * 64;
+      const int2* seen_by = intervals + (2 * w + (k & 1)) * 64;
       bool whole;
       Column ahead;
-      int next_in = in_head + 1, next_hq = hq;
-      if (next_in == count) { next_in = 0; ++next_hq; }
+      const int this_in = in_head, this_hq = hq;
+      in_head += ((u + kUnits) >> 1) - (u >> 1);
+      settle_head();
       if (KV) {
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + h) : "memory");  // the columns are there
-        const int4 q = a.s.mask.q_blocks[(long long)batch * nq + first + in_head];
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");  // the columns are there
+        const int4 q = a.s.mask.q_blocks[(long long)batch * nq + first + this_in];
         whole = q.z <= block * kBlock && q.w >= (block + 1) * kBlock;
-        if (BIAS) slope = a.s.slopes[head * a.s.group + hq] * kLog2e;
-        if (it + 1 < total) ahead = column(next_in, next_hq);
+        if (BIAS) slope = a.s.slopes[head * a.s.group + this_hq] * kLog2e;
+        if (u + kUnits < 2 * total) ahead = column(u + kUnits, in_head, hq);
       } else {
         whole = info.z <= col0 && info.w >= col0 + 64;
       }
-      wait(&bar_s[h], it & 1, 5);
+      wait(&bar_s[w], k & 1, 5);
       const float apart = (float)(KV ? mine - col0 - off : mine + off - col0);  // of this row and column col0
       // 32 columns at a time: P and dS lie over columns that have been read
 #pragma unroll
@@ -875,18 +885,16 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
       wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive(&bar_p[h]);
-      // (the other buffer was last read before this block's barrier)
-      if (KV && it + 1 < total) keep((it + 1) & 1, ahead);
-      in_head = next_in;
-      hq = next_hq;
+      if (lane == 0) arrive(&bar_p[w]);
+      // (the other buffer was last read before this unit's barrier)
+      if (KV && u + kUnits < 2 * total) keep((k + 1) & 1, ahead);
     }
     if (total > 0) wait(bar_a, 0, 6);
-    // dV and dK: one per half of the warps; dQ: half of the columns each
-    const int c_first = KV ? 0 : h * (D / 2), c_last = KV ? D : c_first + D / 2;
-    const uint32_t from = lane_addr + 256u + (uint32_t)(KV ? D * h : 0);
-    const OutTensor out = KV ? (h == 0 ? a.dv : a.dk) : a.dq;
-    const float factor = KV && h == 0 ? 1.f : a.s.scale;
+    // dV and dK: the first eight warps, one each; dQ: half of the columns each
+    const int c_first = KV ? 0 : w * (D / 2), c_last = w > 1 ? c_first : KV ? D : c_first + D / 2;
+    const uint32_t from = lane_addr + kSums + (uint32_t)(KV ? D * w : D);
+    const OutTensor out = KV ? (w == 0 ? a.dv : a.dk) : a.dq;
+    const float factor = KV && w == 0 ? 1.f : a.s.scale;
     const int rows = KV ? a.s.k_len : a.s.q_len;
 #pragma unroll 1
     for (int c = c_first; c < c_last; c += 16) {
@@ -910,14 +918,14 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && *failed != 0 && a.s.status) atomicExch(a.s.status, *failed);
-  if (warp == 9) {
+  if (warp == SM::kMma) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
 }
 
 template <int D, typename T, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(kThreads2, 1)
+__global__ void __launch_bounds__(BwdSmem<D>::kThreads, 1)
 masked_backward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
                        const AttnBwdArgs a) {
@@ -1026,7 +1034,7 @@ int launch_forward(const flb200_attention_desc* d, const CUtensorMap& mq, const 
                    AttnFwdArgs a, cudaStream_t st) {
   const auto kernel = masked_forward_kernel<D, T, CAP, BIAS>;
   if (int rc = configure(reinterpret_cast<const void*>(kernel), FwdSmem<D>::kTotal)) return rc;
-  launch_chained(kernel, (unsigned)(d->batch * d->heads * blocks_of(d->q_len)), kThreads2, FwdSmem<D>::kTotal, st, mq, mk, mv, a);
+  launch_chained(kernel, (unsigned)(d->batch * d->heads * blocks_of(d->q_len)), kFwdThreads, FwdSmem<D>::kTotal, st, mq, mk, mv, a);
   FLB200_AFTER_LAUNCH("masked_attention_forward");
   count_tc_launch();
   return FLB200_OK;
@@ -1038,7 +1046,7 @@ int launch_backward(const flb200_attention_desc* d, const CUtensorMap& mq, const
   if (int rc = configure(reinterpret_cast<const void*>(kernel), BwdSmem<D>::kTotal)) return rc;
   a.kv_ctas = (int)(d->batch * d->kv_heads * blocks_of(d->k_len));
   const unsigned grid = (unsigned)(a.kv_ctas + d->batch * d->heads * blocks_of(d->q_len));
-  launch_chained(kernel, grid, kThreads2, BwdSmem<D>::kTotal, st, mq, mk, mv, mg, a);
+  launch_chained(kernel, grid, BwdSmem<D>::kThreads, BwdSmem<D>::kTotal, st, mq, mk, mv, mg, a);
   FLB200_AFTER_LAUNCH("masked_attention_backward");
   count_tc_launch();
   return FLB200_OK;
