@@ -18,6 +18,7 @@
 #include <cuda_fp8.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 #include "packed.cuh"
@@ -46,20 +47,49 @@ struct AdamwTable {
 constexpr int kSmall = 32, kMiddle = 160, kLarge = 480;
 static_assert(sizeof(AdamwTable<kLarge>) + sizeof(AdamwMath) < 32764, "kernel arguments");
 
-// Eight elements as fp32, of which `live` exist; whole: all do, and p is aligned to them.
+// Eight elements, as they lie in memory where all of them exist and are aligned.
+template <typename T>
+struct alignas(16) Eight {
+  uint32_t w[2 * sizeof(T)];
+};
+template <typename T>
+__device__ __forceinline__ void read8(const T* p, Eight<T>& r) {
+  if constexpr (sizeof(T) == 4) {
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]),
+                   "=r"(r.w[7])
+                 : "l"(p));
+  } else if constexpr (sizeof(T) == 2) {
+    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3])
+                 : "l"(p));
+  } else {
+    asm volatile("ld.global.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(r.w[0]), "=r"(r.w[1]) : "l"(p));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void widen8(const Eight<T>& r, float* v) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) v[j] = __uint_as_float(r.w[j]);
+  } else {
+    unpack16(*reinterpret_cast<const Vec16<T>*>(&r), v);
+  }
+}
+// One by one, of which `live` exist.
+template <typename T>
+__device__ __forceinline__ void load_live(const T* p, int live, float* v) {
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) v[j] = j < live ? Num<T>::to_f(p[j]) : 0.f;
+}
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, bool whole, int live, float* v) {
   if (whole) {
-    if constexpr (sizeof(T) == 4) {
-      asm volatile("ld.global.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                   : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
-                   : "l"(p));
-    } else {
-      unpack16(load16(p), v);
-    }
+    Eight<T> r;
+    read8(p, r);
+    widen8(r, v);
   } else {
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] = j < live ? Num<T>::to_f(p[j]) : 0.f;
+    load_live(p, live, v);
   }
 }
 template <typename T>
@@ -79,26 +109,27 @@ __device__ __forceinline__ void store8(T* p, bool whole, int live, const float* 
   }
 }
 
-// 8-bit states: eight codes, their values over the block's scale
-__device__ __forceinline__ void load_codes(const uint8_t* p, bool whole, int live, float scale, float* v) {
-  uint32_t w[2] = {0, 0};
-  if (whole) {
-    const uint2 c = *reinterpret_cast<const uint2*>(p);
-    w[0] = c.x;
-    w[1] = c.y;
-  } else {
-#pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (j < live) w[j >> 2] |= (uint32_t)p[j] << (8 * (j & 3));
-  }
+// 8-bit states: the values of eight codes over their block's scale
+__device__ __forceinline__ void widen_codes(const Eight<uint8_t>& r, float scale, float* v) {
   const F2 s = pair(scale);
 #pragma unroll
   for (int j = 0; j < kPer; j += 2) {
     const __half2_raw h =
-        __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[j >> 2] >> (8 * (j & 2))), __NV_E4M3);
+        __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(r.w[j >> 2] >> (8 * (j & 2))), __NV_E4M3);
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
     unpair(pair(f.x, f.y) * s, v[j], v[j + 1]);
   }
+}
+__device__ __forceinline__ Eight<uint8_t> codes_live(const uint8_t* p, int live) {
+  Eight<uint8_t> r{{0, 0}};
+#pragma unroll
+  for (int j = 0; j < kPer; ++j)
+    if (j < live) r.w[j >> 2] |= (uint32_t)p[j] << (8 * (j & 3));
+  return r;
+}
+// of numbers that are not negative: their bits are in their order
+__device__ __forceinline__ float warp_top(float v) {
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
 }
 // The warp's block: its scale, and the codes of its values.  kRoot: values >= 0 of which none but zero becomes zero.
 template <bool kRoot>
@@ -106,7 +137,7 @@ __device__ __forceinline__ void store_codes(uint8_t* p, float* scale, bool whole
   float top = 0.f;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) top = fmaxf(top, kRoot ? v[j] : fabsf(v[j]));  // (past the end: zeros)
-  top = fmaxf(warp_max(top), 1e-30f);
+  top = fmaxf(warp_top(top), 1e-30f);
   const float to_code = __fmul_rn(__frcp_rn(top), 448.f);
   const F2 k = pair(to_code);
   uint32_t w[2] = {0, 0};
@@ -131,37 +162,104 @@ __device__ __forceinline__ void store_codes(uint8_t* p, float* scale, bool whole
   if ((threadIdx.x & 31) == 0) *scale = __fmul_rn(top, 1.f / 448.f);
 }
 
+// Where a warp is: its block of 256 elements of tensor `at`, and this lane's eight of them.
+struct Place {
+  int at, live;
+  bool exists, whole;  // of the warp; eight elements that can be read at once
+  long long block, i;
+};
+template <int CAP>
+__device__ __forceinline__ Place place_of(const AdamwTable<CAP>& table, unsigned chunk, int from) {
+  Place x;
+  x.at = from;  // (a CTA's chunks only grow)
+  int hi = table.count;
+  while (hi - x.at > 1) {  // the last tensor that begins at or before this chunk
+    const int mid = (x.at + hi) >> 1;
+    if (table.first_chunk[mid] <= chunk) x.at = mid;
+    else hi = mid;
+  }
+  x.block = (long long)(chunk - table.first_chunk[x.at]) * 8 + (threadIdx.x >> 5);
+  x.i = x.block * kStateBlock + (threadIdx.x & 31) * kPer;
+  const long long n = table.t[x.at].n, left = n - x.i;
+  x.exists = x.block * kStateBlock < n;
+  x.live = left >= kPer ? kPer : (left > 0 ? (int)left : 0);
+  x.whole = x.live == kPer && (table.vec[x.at >> 5] >> (x.at & 31) & 1u);
+  return x;
+}
+template <typename TP, typename TG, typename TS>
+struct Read {
+  Eight<TP> p;
+  Eight<TG> g;
+  Eight<TS> m, v;
+  float m_scale, v_scale;
+};
+
+// With 8-bit states, whose conversions are most of the work, a chunk is read while the one before it is computed
+// (10^9 elements in 16 bits: 3111 us without, 2560 with).  With 32-bit states the warps that fit without those
+// registers keep memory busy (134 10^6 elements: 565 us, with chunks read ahead 608).
 template <typename TP, typename TG, int BITS, int CAP>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, BITS == 8 ? 3 : 1)
 adamw_kernel(const __grid_constant__ AdamwTable<CAP> table, const AdamwMath k) {
   chain_begin();
+  using TS = std::conditional_t<BITS == 8, uint8_t, float>;
   const unsigned chunks = table.first_chunk[table.count];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int at = 0;
-  for (unsigned chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-    // the last tensor that begins at or before this chunk (chunks of a CTA only grow)
-    int hi = table.count;
-    while (hi - at > 1) {
-      const int mid = (at + hi) >> 1;
-      if (table.first_chunk[mid] <= chunk) at = mid;
-      else hi = mid;
+  Read<TP, TG, TS> next;
+  auto read = [&](const Place& x, Read<TP, TG, TS>& r) {
+    const flb200_adamw_tensor& t = table.t[x.at];
+    if (x.whole) {
+      read8(static_cast<const TP*>(t.param) + x.i, r.p);
+      read8(static_cast<const TG*>(t.grad) + x.i, r.g);
+      read8(static_cast<const TS*>(t.first) + x.i, r.m);
+      read8(static_cast<const TS*>(t.second) + x.i, r.v);
     }
-    const flb200_adamw_tensor& t = table.t[at];
-    const long long block = (long long)(chunk - table.first_chunk[at]) * 8 + warp;  // of 256 elements
-    const long long i = block * kStateBlock + lane * kPer;
-    if (block * kStateBlock >= t.n) continue;  // (all lanes of the warp)
-    const long long left = t.n - i;
-    const int live = left >= kPer ? kPer : (left > 0 ? (int)left : 0);
-    const bool whole = live == kPer && (table.vec[at >> 5] >> (at & 31) & 1u);
+    if (BITS == 8 && x.exists) {
+      r.m_scale = t.first_scale[x.block];
+      r.v_scale = t.second_scale[x.block];
+    }
+  };
+  Place there{};
+  int from = 0;
+  if (BITS == 8 && blockIdx.x < chunks) {
+    there = place_of(table, blockIdx.x, 0);
+    read(there, next);
+  }
+  for (unsigned chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+    Place here;
+    Read<TP, TG, TS> now;
+    if constexpr (BITS == 8) {
+      here = there;
+      now = next;
+      if (chunk + gridDim.x < chunks) {
+        there = place_of(table, chunk + gridDim.x, here.at);
+        read(there, next);
+      }
+    } else {
+      here = place_of(table, chunk, from);
+      from = here.at;
+    }
+    if (!here.exists) continue;  // (all lanes of the warp)
+    const flb200_adamw_tensor& t = table.t[here.at];
+    const long long i = here.i, block = here.block;
+    const int live = here.live;
+    const bool whole = here.whole;
     float p[kPer], g[kPer], m[kPer], v[kPer];
-    load8(static_cast<const TP*>(t.param) + i, whole, live, p);
-    load8(static_cast<const TG*>(t.grad) + i, whole, live, g);
     if constexpr (BITS == 32) {
+      load8(static_cast<const TP*>(t.param) + i, whole, live, p);
+      load8(static_cast<const TG*>(t.grad) + i, whole, live, g);
       load8(static_cast<const float*>(t.first) + i, whole, live, m);
       load8(static_cast<const float*>(t.second) + i, whole, live, v);
     } else {
-      load_codes(static_cast<const uint8_t*>(t.first) + i, whole, live, t.first_scale[block], m);
-      load_codes(static_cast<const uint8_t*>(t.second) + i, whole, live, t.second_scale[block], v);
+      if (whole) {
+        widen8(now.p, p);
+        widen8(now.g, g);
+      } else {
+        load_live(static_cast<const TP*>(t.param) + i, live, p);
+        load_live(static_cast<const TG*>(t.grad) + i, live, g);
+        now.m = codes_live(static_cast<const uint8_t*>(t.first) + i, live);
+        now.v = codes_live(static_cast<const uint8_t*>(t.second) + i, live);
+      }
+      widen_codes(now.m, now.m_scale, m);
+      widen_codes(now.v, now.v_scale, v);
     }
     // Each operation of the moments rounds by itself (no contraction): what is kept in 8 bits then depends on
     // the formula alone.
@@ -218,7 +316,7 @@ int launch_adamw(const AdamwMath& math, const flb200_adamw_tensor* tensors, int6
     table.first_chunk[table.count] = (unsigned)chunks;
   }
   if (chunks == 0) return FLB200_OK;
-  const long long cap = 8LL * 4 * device_info().sm_count;
+  const long long cap = 8LL * (BITS == 8 ? 1 : 4) * device_info().sm_count;
   launch_chained(adamw_kernel<TP, TG, BITS, CAP>, (unsigned)(chunks < cap ? chunks : cap), 256, 0, st, table, math);
   FLB200_AFTER_LAUNCH("adamw_step");
   return FLB200_OK;
