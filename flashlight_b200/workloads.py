@@ -243,13 +243,27 @@ class TransformerLM(nn.Module):
     projections, vocabulary projection and all their gradients), LayerNorm statistics, GELU,
     logSoftmax, the loss, the residual adds and the embedding lookup with its scatter-add
     gradient and the scaled causal softmax run on this library's kernels; head split / merge
-    permutations are torch data movement (autograd.glue); nothing arithmetic is left to torch."""
+    permutations are torch data movement (autograd.glue); nothing arithmetic is left to torch.
+
+    packed=True trains on rows that hold several documents (16-bit compute_dtype): a position attends to its own
+    document (autograd.masked_attention_packed; one mask per batch for all layers), and the loss is taken without the
+    scores of the vocabulary in memory (autograd.linear_cross_entropy; targets of -1 do not count).  With it, kv_heads:
+    key and value heads that several query heads share; softcap: scores capped by a tanh; distance_bias: each head's
+    scores fall linearly with the distance, by 2^(-8 (h + 1) / heads) a position."""
 
     def __init__(self, vocab=32000, d=768, heads=12, ffn=3072, layers=12, seed=1234, device="cuda",
-                 compute_dtype=torch.float32):
+                 compute_dtype=torch.float32, packed=False, kv_heads=None, softcap=0.0, distance_bias=False):
         super().__init__()
         gen = torch.Generator().manual_seed(seed)
         self.d, self.heads, self.layers = d, heads, layers
+        self.packed, self.softcap = packed, softcap
+        self.kv_heads = heads if kv_heads is None else kv_heads
+        if not packed and (self.kv_heads != heads or softcap or distance_bias):
+            raise ValueError("TransformerLM: kv_heads, softcap and distance_bias belong to packed=True")
+        if packed and compute_dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("TransformerLM: packed rows are computed in 16 bits")
+        self.slopes = (torch.tensor([2.0 ** (-8.0 * (h + 1) / heads) for h in range(heads)], device=device)
+                       if distance_bias else None)
         # bf16 compute with fp32 master weights: parameters stay fp32; the matrices and the
         # embedding are cast to bf16 where they are used and their gradients come back as fp32
         # (autograd.cast); biases and LayerNorm parameters are used in fp32 by the kernels or
@@ -262,7 +276,7 @@ class TransformerLM(nn.Module):
         self.params = [self.embed]
         self.blocks = []
         for _ in range(layers):
-            blk = {"ln1": (ones(d), zeros(d)), "qkv": mk(d, 3 * d), "proj": mk(d, d),
+            blk = {"ln1": (ones(d), zeros(d)), "qkv": mk(d, d + 2 * self.kv_heads * (d // heads)), "proj": mk(d, d),
                    "ln2": (ones(d), zeros(d)), "w1": mk(d, ffn), "w2": mk(ffn, d)}
             self.blocks.append(blk)
             self.params += list(blk["ln1"]) + list(blk["ln2"])
@@ -296,6 +310,9 @@ class TransformerLM(nn.Module):
         d, h = self.d, self.heads
         hd = d // h
         qkv = self._lin(blk["qkv"], x)  # (B*T, 3d)
+        if mask is not None:
+            return self._lin(blk["proj"], A.masked_attention_packed(
+                qkv, h, mask, 1.0 / math.sqrt(hd), self.softcap, self.slopes, self.kv_heads))
         # one kernel each way on the packed projection where it is built (bf16, head dim 64)
         ctx = A.attention_packed(qkv, B, T, h, 1.0 / math.sqrt(hd), True)
         if ctx is not None:
@@ -316,14 +333,22 @@ class TransformerLM(nn.Module):
             lambda g: _reorder(g, (B, T, h, hd), (0, 2, 1, 3)).reshape(B * h, T, hd))
         return self._lin(blk["proj"], merged)
 
-    def loss(self, ids: torch.Tensor, targets: torch.Tensor) -> Variable:
-        """ids (B, T) token ids; targets (B*T,) next-token labels."""
+    def loss(self, ids: torch.Tensor, targets: torch.Tensor, documents: Optional[torch.Tensor] = None,
+             prefix: Optional[torch.Tensor] = None) -> Variable:
+        """ids (B, T) token ids; targets (B*T,) next-token labels.  With packed=True: documents (B, T) int32, the
+        document of each position, -1 for padding; prefix (B,) int32, positions that all of their document see."""
         B, T = ids.shape
+        if not self.packed and (documents is not None or prefix is not None):
+            raise ValueError("TransformerLM: documents and prefix belong to packed=True")
         x = A.embedding(A.cast(self.embed, self.compute_dtype), ids)  # (B*T, d)
-        mask = None
+        mask = (F.attention_mask(B, T, documents=documents, prefix=prefix, device=ids.device)
+                if self.packed else None)
         for blk in self.blocks:
             x = A.add(x, self._attention(self._ln(x, blk["ln1"]), blk, B, T, mask))
             h = self._lin(blk["w1"], self._ln(x, blk["ln2"]), gelu=True)  # Linear + bias + GELU
             x = A.add(x, self._lin(blk["w2"], h))
+        if self.packed:
+            return A.linear_cross_entropy(self._ln(x, self.ln_f), A.cast(self.head.params[0], self.compute_dtype),
+                                          self.head.params[1], targets)
         scores = self._lin(self.head, self._ln(x, self.ln_f))
         return A.log_softmax_cross_entropy(scores, targets, wide=True)
