@@ -380,8 +380,9 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int nq = blocks_of(a.s.q_len), off = a.s.k_len - a.s.q_len;
-  const int i = nq - 1 - (int)blockIdx.x % nq;  // the longest of a causal head first
-  const int bh = blockIdx.x / nq, batch = bh / a.s.heads, head = bh - batch * a.s.heads;
+  const int all_heads = gridDim.x / nq;
+  const int i = nq - 1 - (int)blockIdx.x / all_heads;  // of all heads the longest of a causal mask first
+  const int bh = blockIdx.x % all_heads, batch = bh / a.s.heads, head = bh - batch * a.s.heads;
   const int4 info = a.s.mask.q_blocks[(long long)batch * nq + i];
   const int begin = info.y > info.x ? info.x / kBlock : 0;
   const int blocks = info.y > info.x ? blocks_of(info.y) - begin : 0;
@@ -658,8 +659,10 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int nq = blocks_of(a.s.q_len), nk = blocks_of(a.s.k_len), off = a.s.k_len - a.s.q_len;
   const int per_head = KV ? nk : nq, heads = KV ? a.s.heads / a.s.group : a.s.heads;
-  const int block = KV ? cta % per_head : per_head - 1 - cta % per_head;  // (the longest of a causal head first)
-  const int bh = cta / per_head, batch = bh / heads, head = bh - batch * heads;
+  const int all_heads = (KV ? a.kv_ctas : (int)gridDim.x - a.kv_ctas) / per_head;
+  // (of all heads the longest of a causal mask first)
+  const int block = KV ? cta / all_heads : per_head - 1 - cta / all_heads;
+  const int bh = cta % all_heads, batch = bh / heads, head = bh - batch * heads;
   int first, count, total;  // column blocks, and how many there are over all heads
   int4 info = make_int4(0, 0, 0, 0);
   if (KV) {
