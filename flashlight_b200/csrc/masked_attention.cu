@@ -301,29 +301,49 @@ __device__ __forceinline__ void load_tile(const CUtensorMap* map, uint64_t* bar,
 struct OutTensor {  // element (batch b, row t, head h, d) at b * batch + t * row + h * head + d
   void* p;
   long long batch, row, head;
+  int wide;  // 16 elements of a row are a sector of 32 bytes
 };
-// 16 columns from c0 on of a row, of which those in front of head_dim exist.  rest (its row, or null) gets what the
-// rounding took: out + rest is right to 2^-16, which D is taken from.  (From out alone D carries a rounding
+template <typename T>
+__device__ __forceinline__ void store_32(T* to, const Vec16<T>& a, const Vec16<T>& b) {
+  const uint4 x = *reinterpret_cast<const uint4*>(&a), y = *reinterpret_cast<const uint4*>(&b);
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(x.x), "r"(x.y), "r"(x.z),
+               "r"(x.w), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w)
+               : "memory");
+}
+// 16 columns from c0 on of a row, of which those in front of head_dim exist.  rest (its row, or null; as wide as o) gets
+// what the rounding took: out + rest is right to 2^-16, which D is taken from.  (From out alone D carries a rounding
 // of |do||o|, and the scores' gradient half as much error again.)
 template <typename T>
 __device__ __forceinline__ void store16_of(const OutTensor& o, int b, int t, int h, int c0, int head_dim,
                                            const uint32_t* v, float factor, T* rest) {
   T* to = static_cast<T*>(o.p) + b * o.batch + t * o.row + h * o.head + c0;
+  float x[16];
+  Vec16<T> r[2];
 #pragma unroll
-  for (int u = 0; u < 16; u += 8)
-    if (c0 + u < head_dim) {
-      float x[8], y[8];
+  for (int e = 0; e < 16; ++e) x[e] = __uint_as_float(v[e]) * factor;
+  r[0] = pack16<T>(x);
+  r[1] = pack16<T>(x + 8);
+  if (o.wide) {
+    if (c0 < head_dim) store_32(to, r[0], r[1]);
+  } else {
+    if (c0 < head_dim) store16(to, r[0]);
+    if (c0 + 8 < head_dim) store16(to + 8, r[1]);
+  }
+  if (rest) {
+    float y[16];
+    unpack16(r[0], y);
+    unpack16(r[1], y + 8);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(v[u + e]) * factor;
-      const Vec16<T> r = pack16<T>(x);
-      store16(to + u, r);
-      if (rest) {
-        unpack16(r, y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = x[e] - y[e];
-        store16(rest + c0 + u, pack16<T>(y));
-      }
+    for (int e = 0; e < 16; ++e) y[e] = x[e] - y[e];
+    r[0] = pack16<T>(y);
+    r[1] = pack16<T>(y + 8);
+    if (o.wide) {
+      if (c0 < head_dim) store_32(rest + c0, r[0], r[1]);
+    } else {
+      if (c0 < head_dim) store16(rest + c0, r[0]);
+      if (c0 + 8 < head_dim) store16(rest + c0 + 8, r[1]);
     }
+  }
 }
 
 struct AttnShape {
@@ -387,7 +407,18 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   const int begin = info.y > info.x ? info.x / kBlock : 0;
   const int blocks = info.y > info.x ? blocks_of(info.y) - begin : 0;
 
-  if (threadIdx.x == 0) {
+  const int kv = head / a.s.group;
+  auto load = [&](int j, uint32_t s, bool k, bool v) {
+    if (k) {
+      mbar_expect_tx(&k_full[s], kTile);
+      load_tile<D>(&map_k, &k_full[s], sK + s * kTile, j * kBlock, kv, batch);
+    }
+    if (v) {
+      mbar_expect_tx(&v_full[s], kTile);
+      load_tile<D>(&map_v, &v_full[s], sV + s * kTile, j * kBlock, kv, batch);
+    }
+  };
+  if (warp == 8 && elect_one()) {
     mbar_init(bar_q, 1);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&k_full[s], 1);
@@ -400,6 +431,11 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     mbar_init(bar_o, 1);
     *failed = 0;
     fence_barrier_init();
+    if (blocks > 0) {  // (the first copies run while tensor memory is allocated)
+      mbar_expect_tx(bar_q, kTile);
+      load_tile<D>(&map_q, bar_q, sQ, i * kBlock, head, batch);
+      load(begin, 0, true, true);
+    }
   }
   if (warp == 9) tmem_alloc(tmem_slot, 256);
   tc_fence_before();
@@ -412,18 +448,13 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   };
 
   if (warp == 8) {
-    if (blocks > 0 && elect_one()) {
-      mbar_expect_tx(bar_q, kTile);
-      load_tile<D>(&map_q, bar_q, sQ, i * kBlock, head, batch);
-      const int kv = head / a.s.group;
-      uint32_t s = 0, round = 0;
-      for (int j = begin; j < begin + blocks; ++j) {
+    if (blocks > 1 && elect_one()) {
+      uint32_t s = kStages == 1 ? 0 : 1, round = kStages == 1 ? 1 : 0;
+      for (int j = begin + 1; j < begin + blocks; ++j) {
         if (round > 0) wait(&k_empty[s], (round - 1) & 1, 1);
-        mbar_expect_tx(&k_full[s], kTile);
-        load_tile<D>(&map_k, &k_full[s], sK + s * kTile, j * kBlock, kv, batch);
+        load(j, s, true, false);
         if (round > 0) wait(&v_empty[s], (round - 1) & 1, 2);
-        mbar_expect_tx(&v_full[s], kTile);
-        load_tile<D>(&map_v, &v_full[s], sV + s * kTile, j * kBlock, kv, batch);
+        load(j, s, false, true);
         if (++s == kStages) { s = 0; ++round; }
       }
     }
@@ -618,14 +649,16 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 //     P and dS over the same columns, 16 bits, A operands of
 //     dV += P cols2, dK += dS cols1   or   dQ += dS cols1     (the last 2 D columns)
 // What bounds a unit is its chain from contraction to P and dS to contraction, so as many units are under way as tensor
-// memory holds: three at 64 dimensions, two at 128.
+// memory holds: three at 64 dimensions (or one in each of two CTAs, see launch_backward), two at 128.
 // Nothing is added across CTAs: the result does not depend on their order.  The price is that S and dP are made
 // twice, 7 contractions where sums in device memory need 5; those would cost 4 bytes a value per key block.
-template <int D>
+template <int D, int UNITS>
 struct BwdSmem {
-  static constexpr int kUnits = D == 64 ? 3 : 2;  // under way: four warps, and 128 columns of tensor memory, each
+  static constexpr int kUnits = UNITS;  // under way: four warps, and 128 columns of tensor memory, each
+  static constexpr int kTmem = UNITS == 1 ? 256 : 512;
+  static_assert(128 * UNITS + 2 * D <= kTmem, "tensor memory");
   // (the unit that is issued behind the last of a block lies up to kUnits / 2 blocks further)
-  static constexpr int kTile = D / 64 * kBox, kStages = D == 64 ? 3 : 2;
+  static constexpr int kTile = D / 64 * kBox, kStages = UNITS == 3 ? 3 : 2;
   static constexpr int kThreads = (4 * kUnits + 2) * 32, kTma = 4 * kUnits, kMma = kTma + 1;  // (the last two warps)
   static constexpr int kColumns = kUnits * 2 * 64 * 16;  // two buffers of lse, D and interval per query column
   static constexpr int kTotal = 2 * kTile + 2 * kStages * kTile + kColumns + 1024 + 256;
@@ -638,13 +671,13 @@ struct AttnBwdArgs {
   int kv_ctas;        // the first of the grid: dK and dV
 };
 
-template <int D, typename T, bool CAP, bool BIAS, bool KV>
+template <int D, int UNITS, typename T, bool CAP, bool BIAS, bool KV>
 __device__ __forceinline__ void
 backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, const CUtensorMap& map_do,
               const AttnBwdArgs& a, int cta) {
-  using SM = BwdSmem<D>;
+  using SM = BwdSmem<D, UNITS>;
   constexpr int kStages = SM::kStages, kTile = SM::kTile, kUnits = SM::kUnits;
-  constexpr uint32_t kSums = 512 - 2 * D;  // first column of the sums
+  constexpr uint32_t kSums = SM::kTmem - 2 * D;  // first column of the sums
   extern __shared__ __align__(1024) char smem_raw[];
   char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   char *sR1 = base, *sR2 = base + kTile, *sC1 = base + 2 * kTile, *sC2 = sC1 + kStages * kTile;
@@ -677,7 +710,13 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
     total = count;
   }
 
-  if (threadIdx.x == 0) {
+  auto load = [&](uint32_t s, int b, int h) {
+    mbar_expect_tx(&full[s], 2 * kTile);
+    load_tile<D>(KV ? &map_q : &map_k, &full[s], sC1 + s * kTile, b * kBlock, h, batch);
+    load_tile<D>(KV ? &map_do : &map_v, &full[s], sC2 + s * kTile, b * kBlock, h, batch);
+  };
+  const int first_head = KV ? head * a.s.group : head / a.s.group;  // of the columns
+  if (warp == SM::kTma && elect_one()) {
     mbar_init(bar_r, 1);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
@@ -690,8 +729,14 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
     mbar_init(bar_a, 1);
     *failed = 0;
     fence_barrier_init();
+    if (total > 0) {  // (the first copies run while tensor memory is allocated)
+      mbar_expect_tx(bar_r, 2 * kTile);
+      load_tile<D>(KV ? &map_k : &map_q, bar_r, sR1, block * kBlock, head, batch);
+      load_tile<D>(KV ? &map_v : &map_do, bar_r, sR2, block * kBlock, head, batch);
+      load(0, first, first_head);
+    }
   }
-  if (warp == SM::kMma) tmem_alloc(tmem_slot, 512);
+  if (warp == SM::kMma) tmem_alloc(tmem_slot, SM::kTmem);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -702,19 +747,14 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
   };
 
   if (warp == SM::kTma) {
-    if (total > 0 && elect_one()) {
-      mbar_expect_tx(bar_r, 2 * kTile);
-      load_tile<D>(KV ? &map_k : &map_q, bar_r, sR1, block * kBlock, head, batch);
-      load_tile<D>(KV ? &map_v : &map_do, bar_r, sR2, block * kBlock, head, batch);
-      uint32_t s = 0, round = 0;
-      int in_head = 0, h = KV ? head * a.s.group : head / a.s.group;
-      for (int it = 0; it < total; ++it) {
+    if (total > 1 && elect_one()) {
+      uint32_t s = 1, round = 0;
+      int in_head = 1, h = first_head;
+      for (int it = 1; it < total; ++it) {
+        if (in_head == count) { in_head = 0; ++h; }
         if (round > 0) wait(&empty[s], (round - 1) & 1, 1);
-        mbar_expect_tx(&full[s], 2 * kTile);
-        load_tile<D>(KV ? &map_q : &map_k, &full[s], sC1 + s * kTile, (first + in_head) * kBlock, h, batch);
-        load_tile<D>(KV ? &map_do : &map_v, &full[s], sC2 + s * kTile, (first + in_head) * kBlock, h, batch);
+        load(s, first + in_head++, h);
         if (++s == kStages) { s = 0; ++round; }
-        if (++in_head == count) { in_head = 0; ++h; }
       }
     }
   } else if (warp == SM::kMma) {
@@ -893,18 +933,14 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
       if (KV && u + kUnits < 2 * total) keep((k + 1) & 1, ahead);
     }
     if (total > 0) wait(bar_a, 0, 6);
-    // dV and dK: the first eight warps, one each; dQ: half of the columns each
-    const int c_first = KV ? 0 : w * (D / 2), c_last = w > 1 ? c_first : KV ? D : c_first + D / 2;
-    const uint32_t from = lane_addr + kSums + (uint32_t)(KV ? D * w : D);
-    const OutTensor out = KV ? (w == 0 ? a.dv : a.dk) : a.dq;
-    const float factor = KV && w == 0 ? 1.f : a.s.scale;
+    // dV and dK, 2 D columns of sums, or dQ, the last D: 16 columns at a time, in turn
     const int rows = KV ? a.s.k_len : a.s.q_len;
 #pragma unroll 1
-    for (int c = c_first; c < c_last; c += 16) {
+    for (int c = (KV ? 0 : D) + 16 * w; c < 2 * D; c += 16 * kUnits) {
       uint32_t o[16];
       __syncwarp();
       if (total > 0) {
-        ld16_begin(from + c, o);
+        ld16_begin(lane_addr + kSums + c, o);
         wait_ld();
         settle16(o);
       } else {
@@ -912,7 +948,8 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
         for (int e = 0; e < 16; ++e) o[e] = 0;
       }
       if (mine < rows)
-        store16_of<T>(out, batch, mine, head, c, a.s.head_dim, o, factor, nullptr);
+        store16_of<T>(KV ? (c < D ? a.dv : a.dk) : a.dq, batch, mine, head, c & (D - 1), a.s.head_dim, o,
+                      c < D ? 1.f : a.s.scale, nullptr);
     }
   }
   if (*failed)
@@ -923,30 +960,30 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
   if (threadIdx.x == 0 && *failed != 0 && a.s.status) atomicExch(a.s.status, *failed);
   if (warp == SM::kMma) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, SM::kTmem);
   }
 }
 
-template <int D, typename T, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(BwdSmem<D>::kThreads, 1)
+template <int D, int UNITS, typename T, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(BwdSmem<D, UNITS>::kThreads, UNITS == 1 ? 2 : 1)
 masked_backward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
                        const AttnBwdArgs a) {
   chain_begin();
   if ((int)blockIdx.x < a.kv_ctas)
-    backward_body<D, T, CAP, BIAS, true>(map_q, map_k, map_v, map_do, a, blockIdx.x);
+    backward_body<D, UNITS, T, CAP, BIAS, true>(map_q, map_k, map_v, map_do, a, blockIdx.x);
   else
-    backward_body<D, T, CAP, BIAS, false>(map_q, map_k, map_v, map_do, a, blockIdx.x - a.kv_ctas);
+    backward_body<D, UNITS, T, CAP, BIAS, false>(map_q, map_k, map_v, map_do, a, blockIdx.x - a.kv_ctas);
 }
 
-// D = rowsum(dO * (O + rest)): sixteen lanes per row, one 16-byte load each.  Results in [batch][heads][q_len].
-template <typename T>
+// D = rowsum(dO * (O + rest)): LANES lanes per row, one 16-byte load of each.  Results in [batch][heads][q_len].
+template <typename T, int LANES>
 __global__ void __launch_bounds__(256)
 masked_dsum_kernel(const OutTensor o, const T* __restrict__ rest, const OutTensor go, float* __restrict__ dsum,
                    long long rows, int q_len, int heads, int head_dim) {
   chain_begin();
-  const long long t = blockIdx.x * 256LL + threadIdx.x, r = t >> 4;
-  const int c = 8 * (int)(t & 15);
+  const long long t = blockIdx.x * 256LL + threadIdx.x, r = t / LANES;
+  const int c = 8 * (int)(t % LANES);
   float acc = 0.f;
   long long bt = 0, b = 0;
   int h = 0;
@@ -970,7 +1007,7 @@ masked_dsum_kernel(const OutTensor o, const T* __restrict__ rest, const OutTenso
     }
   }
 #pragma unroll
-  for (int k = 1; k < 16; k <<= 1) acc += __shfl_xor_sync(0xffffffffu, acc, k);
+  for (int k = 1; k < LANES; k <<= 1) acc += __shfl_xor_sync(0xffffffffu, acc, k);
   if (r < rows && c == 0) dsum[(b * heads + h) * q_len + bt - b * q_len] = acc;
 }
 
@@ -993,7 +1030,11 @@ int configure(const void* kernel, int smem) {
   done.insert({dev, kernel});
   return FLB200_OK;
 }
-OutTensor out_of(const flb200_head_tensor& t) { return OutTensor{t.data, t.batch, t.row, t.head}; }
+OutTensor out_of(const flb200_head_tensor& t, long long head_dim) {
+  const bool wide = (reinterpret_cast<uintptr_t>(t.data) & 31) == 0 &&
+                    (t.batch | t.row | t.head | head_dim) % 16 == 0;
+  return OutTensor{t.data, t.batch, t.row, t.head, wide ? 1 : 0};
+}
 
 AttnShape shape_of(const flb200_attention_desc* d, const float* slopes, const void* mask) {
   AttnShape s{};
@@ -1042,17 +1083,32 @@ int launch_forward(const flb200_attention_desc* d, const CUtensorMap& mq, const 
   count_tc_launch();
   return FLB200_OK;
 }
-template <int D, typename T, bool CAP, bool BIAS>
-int launch_backward(const flb200_attention_desc* d, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                    const CUtensorMap& mg, AttnBwdArgs a, cudaStream_t st) {
-  const auto kernel = masked_backward_kernel<D, T, CAP, BIAS>;
-  if (int rc = configure(reinterpret_cast<const void*>(kernel), BwdSmem<D>::kTotal)) return rc;
+template <int D, int UNITS, typename T, bool CAP, bool BIAS>
+int launch_backward_as(const flb200_attention_desc* d, const CUtensorMap& mq, const CUtensorMap& mk,
+                       const CUtensorMap& mv, const CUtensorMap& mg, AttnBwdArgs a, cudaStream_t st) {
+  using SM = BwdSmem<D, UNITS>;
+  const auto kernel = masked_backward_kernel<D, UNITS, T, CAP, BIAS>;
+  if (int rc = configure(reinterpret_cast<const void*>(kernel), SM::kTotal)) return rc;
   a.kv_ctas = (int)(d->batch * d->kv_heads * blocks_of(d->k_len));
   const unsigned grid = (unsigned)(a.kv_ctas + d->batch * d->heads * blocks_of(d->q_len));
-  launch_chained(kernel, grid, BwdSmem<D>::kThreads, BwdSmem<D>::kTotal, st, mq, mk, mv, mg, a);
+  launch_chained(kernel, grid, SM::kThreads, SM::kTotal, st, mq, mk, mv, mg, a);
   FLB200_AFTER_LAUNCH("masked_attention_backward");
   count_tc_launch();
   return FLB200_OK;
+}
+template <int D, typename T, bool CAP, bool BIAS>
+int launch_backward(const flb200_attention_desc* d, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+                    const CUtensorMap& mg, const AttnBwdArgs& a, cudaStream_t st) {
+  if constexpr (D == 64) {
+    // Short rows are bound by what a CTA does before its first and after its last unit, which a second CTA on the SM
+    // fills; long ones by the units under way, of which one CTA holds three and two CTAs one each.  12 heads of 8 x 512,
+    // documents of 128: 28 us with two CTAs, 37 with one; 16 of 2 x 4096 316 and 308, in documents of 1000
+    // 145 and 156; 16 of 8192 562 and 521.
+    if (d->k_len <= 4096) return launch_backward_as<D, 1, T, CAP, BIAS>(d, mq, mk, mv, mg, a, st);
+    return launch_backward_as<D, 3, T, CAP, BIAS>(d, mq, mk, mv, mg, a, st);
+  } else {
+    return launch_backward_as<D, 2, T, CAP, BIAS>(d, mq, mk, mv, mg, a, st);
+  }
 }
 // f(std::integral_constant<int, D>, T, cap, bias)
 template <class F>
@@ -1118,8 +1174,9 @@ int flb200_masked_attention_forward(const flb200_attention_desc* d, const flb200
   if (int rc = head_map(&mv, *v, d->batch, d->kv_heads, d->k_len, d->head_dim, operand)) return rc;
   AttnFwdArgs a{};
   a.s = shape_of(d, slopes, mask);
-  a.out = out_of(*out);
+  a.out = out_of(*out, d->head_dim);
   a.rest = rest;
+  if (reinterpret_cast<uintptr_t>(rest) & 31) a.out.wide = 0;
   a.lse = lse;
   return dispatch(d, slopes != nullptr, [&](auto dim, auto type, auto cap, auto bias) {
     return launch_forward<decltype(dim)::value, decltype(type), decltype(cap)::value, decltype(bias)::value>(
@@ -1156,23 +1213,26 @@ int flb200_masked_attention_backward(const flb200_attention_desc* d, const flb20
   if (int rc = head_map(&mg, *grad_out, d->batch, d->heads, d->q_len, d->head_dim, operand)) return rc;
   float* dsum = static_cast<float*>(workspace);
   const long long rows = d->batch * d->heads * d->q_len;
-  const unsigned grid = (unsigned)((rows * 16 + 255) / 256);
-  if (d->dtype == FLB200_F16)
-    launch_chained(masked_dsum_kernel<__half>, grid, 256, 0, st, out_of(*out),
-                   static_cast<const __half*>(rest), out_of(*grad_out), dsum, rows, (int)d->q_len, (int)d->heads,
-                   (int)d->head_dim);
-  else
-    launch_chained(masked_dsum_kernel<__nv_bfloat16>, grid, 256, 0, st, out_of(*out),
-                   static_cast<const __nv_bfloat16*>(rest), out_of(*grad_out), dsum, rows, (int)d->q_len, (int)d->heads,
-                   (int)d->head_dim);
+  const auto row_sums = [&](auto type, auto lanes) {
+    using T = decltype(type);
+    launch_chained(masked_dsum_kernel<T, decltype(lanes)::value>, (unsigned)((rows * lanes + 255) / 256), 256, 0, st,
+                   out_of(*out, d->head_dim), static_cast<const T*>(rest), out_of(*grad_out, d->head_dim), dsum, rows,
+                   (int)d->q_len, (int)d->heads, (int)d->head_dim);
+  };
+  const auto by_lanes = [&](auto type) {
+    if (d->head_dim <= 64) row_sums(type, std::integral_constant<int, 8>{});
+    else row_sums(type, std::integral_constant<int, 16>{});
+  };
+  if (d->dtype == FLB200_F16) by_lanes(__half{});
+  else by_lanes(__nv_bfloat16{});
   FLB200_AFTER_LAUNCH("masked_attention_dsum");
   AttnBwdArgs a{};
   a.s = shape_of(d, slopes, mask);
   a.lse = lse;
   a.dsum = dsum;
-  a.dq = out_of(*grad_q);
-  a.dk = out_of(*grad_k);
-  a.dv = out_of(*grad_v);
+  a.dq = out_of(*grad_q, d->head_dim);
+  a.dk = out_of(*grad_k, d->head_dim);
+  a.dv = out_of(*grad_v, d->head_dim);
   return dispatch(d, slopes != nullptr, [&](auto dim, auto type, auto cap, auto bias) {
     return launch_backward<decltype(dim)::value, decltype(type), decltype(cap)::value, decltype(bias)::value>(
         d, mq, mk, mv, mg, a, st);
