@@ -360,8 +360,10 @@ struct AttnShape {
 // ------------------------------------------------------------------------------------------ forward
 // One CTA takes 128 queries of a head and walks the keys' blocks, two CTAs to an SM: while one is at its softmax the
 // tensor pipe is at the other's products.
-//     S = Q K_j^T    columns 0 ..       P over the same columns, 16 bits, the A operand of
+//     S = Q K_j^T    columns 0 ..       P, 16 bits, the A operand of
 //     O += P V_j     columns 128 ..     (kept over j)
+// At 128 dimensions P lies over S.  At 64 it has columns 192 .. of its own, and the next S is made as soon as all have
+// read this one.
 // Two threads share a row, half of the columns each, and agree on its maximum through shared memory.  P is exp2 of
 // the scores less a reference that is raised, and O rescaled, only where a row's maximum passed it by more than
 // 2^8: rarely behind the first blocks.  P up to 2^8 loses nothing in either type.
@@ -388,14 +390,17 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   chain_begin();
   using SM = FwdSmem<D>;
   constexpr int kStages = SM::kStages, kTile = SM::kTile;
+  constexpr bool kApart = D == 64;                  // P beside S
+  constexpr uint32_t kP = kApart ? 192 : 0;         // its first column
   extern __shared__ __align__(1024) char smem_raw[];
   char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   char *sQ = base, *sK = base + kTile, *sV = sK + kStages * kTile;
   float* exchange = reinterpret_cast<float*>(sV + kStages * kTile);  // [2][2 halves][128 rows]
   uint64_t* bars = reinterpret_cast<uint64_t*>(exchange + 512);
   uint64_t *bar_q = bars, *k_full = bars + 1, *k_empty = k_full + kStages, *v_full = k_empty + kStages,
-           *v_empty = v_full + kStages, *bar_s = v_empty + kStages, *bar_p = bar_s + 1, *bar_o = bar_p + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_o + 1);
+           *v_empty = v_full + kStages, *bar_s = v_empty + kStages, *bar_p = bar_s + 1, *bar_o = bar_p + 1,
+           *bar_read = bar_o + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_read + 1);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -429,6 +434,7 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     mbar_init(bar_s, 1);
     mbar_init(bar_p, 8);
     mbar_init(bar_o, 1);
+    mbar_init(bar_read, 8);
     *failed = 0;
     fence_barrier_init();
     if (blocks > 0) {  // (the first copies run while tensor memory is allocated)
@@ -477,23 +483,27 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       wait(bar_q, 0, 3);
       scores();
       for (int it = 0; it < blocks; ++it) {
+        if (kApart && it + 1 < blocks) {
+          wait(bar_read, it & 1, 7);
+          scores();
+        }
         wait(&v_full[vs], v_round & 1, 6);
         wait(bar_p, it & 1, 5);
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)  // K = 128 keys
-          umma_f16_ts(tmem + 128, tmem + 8 * kk, umma_desc_advance(dV, vs * kTile + kk * 2048), id_o,
+          umma_f16_ts(tmem + 128, tmem + kP + 8 * kk, umma_desc_advance(dV, vs * kTile + kk * 2048), id_o,
                       (it > 0 || kk > 0) ? 1u : 0u);
         umma_commit(bar_o);
         umma_commit(&v_empty[vs]);
         if (++vs == kStages) { vs = 0; ++v_round; }
-        if (it + 1 < blocks) scores();  // (behind the product that reads P, in the pipe's order)
+        if (!kApart && it + 1 < blocks) scores();  // (behind the product that reads P, in the pipe's order)
       }
     }
   } else {
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const int q = i * kBlock + row;
     const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t s_addr = lane_addr + 64u * half, p_addr = lane_addr + 32u * half;
+    const uint32_t s_addr = lane_addr + 64u * half, p_addr = lane_addr + kP + 32u * half;
     const uint32_t o_addr = lane_addr + 128u + (uint32_t)(D / 2 * half);
     int2 seen = make_int2(0, 0);
     if (q < a.s.q_len) seen = a.s.mask.rows[(long long)batch * a.s.q_len + q];
@@ -508,6 +518,11 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       wait_ld();
       settle(s[0]);
       settle(s[1]);
+      if (kApart && it + 1 < blocks) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive(bar_read);
+      }
       // The scores in powers of 2.  (Without cap and bias they stay as they are: the factor is positive and comes
       // with the subtraction below.)
       if constexpr (CAP || BIAS) {
@@ -553,16 +568,17 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       if constexpr (!CAP && !BIAS) mx *= a.s.to_log2;
       float* met = exchange + (it & 1) * 256 + row;
       met[128 * half] = mx;
-      // the two warps that share these rows; behind it P may lie over the scores, which both have read
+      // the two warps that share these rows (behind it P may lie over the scores, which both have read)
       asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
       mx = fmaxf(mx, met[128 * (half ^ 1)]);
+      if (kApart && it > 0) wait(bar_o, (it - 1) & 1, 9);  // the last P has been read
       const bool raise = mx > ref + 8.f;
       if (__any_sync(0xffffffffu, raise)) {
         const float next = raise ? mx : ref, alpha = raise ? ex2(ref - next) : 1.f;
         ref = next;
         sum *= alpha;
         if (it > 0) {
-          wait(bar_o, (it - 1) & 1, 9);
+          if (!kApart) wait(bar_o, (it - 1) & 1, 9);
 #pragma unroll 1
           for (int c = 0; c < D / 2; c += 16) {
             uint32_t o[16];
