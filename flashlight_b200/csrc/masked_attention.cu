@@ -211,6 +211,31 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// 2^z of two numbers below 2^7 on the FMA pipe: Cody and Waite's reduction to [-1/2, 1/2], a polynomial of degree 4 (the
+// one of the least relative error, 2.6e-6, from Remez' exchange), and the exponent added to its bits.  Below -126 the
+// result stays at 2^-126.
+__device__ __forceinline__ void exp2_by_fma(F2 z, float& a, float& b) {
+  float z0, z1, t0, t1;
+  unpair(z, z0, z1);
+  z = pair(fmaxf(z0, -126.f), fmaxf(z1, -126.f));
+  const F2 t = z + pair(12582912.f);  // 1.5 * 2^23: the nearest integer is in the low bits
+  const F2 f = z + fused(t, pair(-1.f), pair(12582912.f));
+  F2 p = fused(f, pair(0.009570102207362652f), pair(0.05591785907745361f));
+  p = fused(p, f, pair(0.240247443318367f));
+  p = fused(p, f, pair(0.6931217908859253f));
+  p = fused(p, f, pair(0.9999992847442627f));
+  unpair(t, t0, t1);
+  unpair(p, a, b);
+  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
+  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
+}
+// One pair of a row's exponentials in this many is made so, the others by the special function unit (0: all).  At 64
+// dimensions that unit is the busiest, at 128 the tensor pipe, but with a cap, which takes two more of it a score.  16 heads of 8192 causal positions, us: forward at 64
+// 195 with none, 190 with one in eight, 182 in four, 206 in two; with a distance bias (12 heads, documents of 3000) 106, 101,
+// 110, 122; gradient 524, 505, 519, 552; forward at 128 246, 258, 268, 276; 2 x 1500 with a cap at 128 forward 57, 49, 53,
+// 60, gradient 150, 128, 142, 144.
+constexpr int forward_by_fma(int D, bool cap, bool bias) { return cap ? 8 : D == 64 ? (bias ? 8 : 4) : 0; }
+constexpr int gradient_by_fma(int D, bool cap) { return D == 64 || cap ? 8 : 0; }
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (std::is_same<T, __half>::value) {
@@ -391,6 +416,7 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   using SM = FwdSmem<D>;
   constexpr int kStages = SM::kStages, kTile = SM::kTile;
   constexpr bool kApart = D == 64;                  // P beside S
+  constexpr int kByFma = forward_by_fma(D, CAP, BIAS);
   constexpr uint32_t kP = kApart ? 192 : 0;         // its first column
   extern __shared__ __align__(1024) char smem_raw[];
   char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -549,7 +575,8 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           }
       }
       // (blocks that all rows see whole need no test per element)
-      if (!(info.z <= key0 && info.w >= key0 + 64)) {
+      const bool whole = info.z <= key0 && info.w >= key0 + 64;
+      if (!whole) {
         const unsigned width = (unsigned)max(seen.y - seen.x, 0);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
@@ -592,23 +619,31 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         }
       }
       F2 sum2 = pair(0.f);
+      const auto exponentials = [&](auto mixed) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t p[16];
+        for (int c = 0; c < 2; ++c) {
+          uint32_t p[16];
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          F2 z = pair(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
-          if constexpr (CAP || BIAS) z = z + pair(-ref);
-          else z = fused(z, pair(a.s.to_log2), pair(-ref));
-          float p0, p1;
-          unpair(z, p0, p1);
-          p0 = ex2(p0);
-          p1 = ex2(p1);
-          sum2 = sum2 + pair(p0, p1);
-          p[e / 2] = pack2<T>(p0, p1);
+          for (int e = 0; e < 32; e += 2) {
+            F2 z = pair(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+            if constexpr (CAP || BIAS) z = z + pair(-ref);
+            else z = fused(z, pair(a.s.to_log2), pair(-ref));
+            float p0, p1;
+            if (kByFma > 0 && decltype(mixed)::value && (e / 2) % (kByFma + !kByFma) == 0) {
+              exp2_by_fma(z, p0, p1);
+            } else {
+              unpair(z, p0, p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+            }
+            sum2 = sum2 + pair(p0, p1);
+            p[e / 2] = pack2<T>(p0, p1);
+          }
+          st16(p_addr + 16 * c, p);
         }
-        st16(p_addr + 16 * c, p);
-      }
+      };
+      if (whole) exponentials(std::true_type{});
+      else exponentials(std::false_type{});  // (what is not seen is zero to the bit)
       float s0, s1;
       unpair(sum2, s0, s1);
       sum += s0 + s1;
@@ -694,6 +729,7 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
   using SM = BwdSmem<D, UNITS>;
   constexpr int kStages = SM::kStages, kTile = SM::kTile, kUnits = SM::kUnits;
   constexpr uint32_t kSums = SM::kTmem - 2 * D;  // first column of the sums
+  constexpr int kByFma = gradient_by_fma(D, CAP);
   extern __shared__ __align__(1024) char smem_raw[];
   char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   char *sR1 = base, *sR2 = base + kTile, *sC1 = base + 2 * kTile, *sC2 = sC1 + kStages * kTile;
@@ -912,9 +948,13 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
               z = fused(z, pair(a.s.to_log2), less);
             }
             float p0, p1, d0, d1;
-            unpair(z, p0, p1);
-            p0 = ex2(p0);
-            p1 = ex2(p1);
+            if (kByFma > 0 && !decltype(tested)::value && (e / 2) % (kByFma + !kByFma) == 0) {
+              exp2_by_fma(z, p0, p1);
+            } else {
+              unpair(z, p0, p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+            }
             F2 d = pair(__uint_as_float(dr[e]), __uint_as_float(dr[e + 1])) + (KV ? pair(-x.y, -x.w) : pair(-my_d));
             d = d * pair(p0, p1);
             if (CAP) d = d * flat;
