@@ -254,6 +254,14 @@ struct SumProblem : GemmProblem<BN> {
   long long ld, split_stride;
   const float* factor;  // or null
   bool vec;
+  // rows of `stride` elements; `by`: factor, `aligned`: rows are aligned to four elements
+  void set(void* to, long long stride, long long splits_apart, const float* by, bool aligned) {
+    out = static_cast<T*>(to);
+    ld = stride;
+    split_stride = splits_apart;
+    factor = by;
+    vec = aligned;
+  }
   __device__ __forceinline__ void store(const typename GemmProblem<BN>::Tile& t, int row, int c0, const float* v,
                                         float* stage, int lane) const {
     const int nb = t.n0 + c0, m_first = t.m0 + row - lane;
@@ -325,8 +333,10 @@ template <int BN> using GradScoreBf16 = GradScoreProblem<BN, __nv_bfloat16>;
 template <int BN> using GradScoreF16 = GradScoreProblem<BN, __half>;
 template <int BN> using SumFirst = SumProblem<BN, float, false>;
 template <int BN> using SumNext = SumProblem<BN, float, true>;
-template <int BN> using WeightBf16 = SumProblem<BN, __nv_bfloat16, false>;
-template <int BN> using WeightF16 = SumProblem<BN, __half, false>;
+template <typename T>
+struct Result16 {
+  template <int BN> using Of = SumProblem<BN, T, false>;
+};
 
 // ------------------------------------------------------------------------------------------ around the products
 // dst [rows][dst_ld] = src [rows][src_ld] of 16-bit values, `cols` of each row and zeros behind them: the copy of
@@ -351,14 +361,35 @@ __device__ __forceinline__ bool counts(int target, int ignore, long long classes
   return target != ignore && target >= 0 && target < classes;
 }
 
+// What a call's rows add up to.
+struct LossSums {
+  double loss;
+  int count, bad;
+};
+// (a lane each of one warp)
+__device__ __forceinline__ LossSums sum_of_warp(LossSums s) {
+  s.loss = warp_sum(s.loss);
+  s.count = __reduce_add_sync(0xffffffffu, s.count);
+  s.bad = __reduce_or_sync(0xffffffffu, s.bad);
+  return s;
+}
+__device__ __forceinline__ void write_loss(const LossSums& s, int reduction, float* loss, int32_t* count,
+                                           int32_t* bad) {
+  if (count) *count = s.count;
+  if (bad) *bad = s.bad;
+  if (reduction == FLB200_REDUCE_MEAN) loss[0] = (float)(s.loss / (double)s.count);
+  else if (reduction == FLB200_REDUCE_SUM) loss[0] = (float)s.loss;
+}
+
 // Joins the tiles' (maximum, sum) of 32 rows per CTA: 32 threads to a row take every 32nd part and meet in shared
-// memory (with eight to a row 13 us for 4096 rows of 250 parts).  Then the rows' losses, and their sum and count per CTA.
+// memory (with eight to a row 13 us for 4096 rows of 250 parts, so 7).  Then the rows' losses, and what they add up to:
+// of all rows where there is one CTA, else finish_loss_kernel adds the CTAs'.
 constexpr int kJoin = 32;
 __global__ void __launch_bounds__(32 * kJoin)
 join_lse_kernel(const float2* __restrict__ partial, int parts, const float* __restrict__ target_score,
-                const int32_t* __restrict__ targets, int ignore, long long classes, int rows,
-                float* __restrict__ lse, float* __restrict__ loss_none, double2* __restrict__ sums,
-                int32_t* __restrict__ bad) {
+                const int32_t* __restrict__ targets, int ignore, long long classes, int rows, int reduction,
+                float* __restrict__ lse, float* __restrict__ loss, int32_t* __restrict__ count,
+                int32_t* __restrict__ bad, LossSums* __restrict__ sums) {
   chain_begin();
   __shared__ float2 met[kJoin][32];
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, r = blockIdx.x * 32 + lane;
@@ -384,7 +415,7 @@ join_lse_kernel(const float2* __restrict__ partial, int parts, const float* __re
     }
   }
   if (g > 0) return;
-  double loss = 0.0, n = 0.0;
+  LossSums all{0.0, 0, 0};
   if (r < rows) {
     const float l = top + logf(sum);
     lse[r] = l;
@@ -392,34 +423,32 @@ join_lse_kernel(const float2* __restrict__ partial, int parts, const float* __re
     float mine = 0.f;
     if (counts(t, ignore, classes)) {
       mine = l - target_score[r];
-      n = 1.0;
-    } else if (t != ignore && bad) {
-      atomicOr(bad, 1);
+      all.count = 1;
+    } else if (t != ignore) {
+      all.bad = 1;
     }
-    if (loss_none) loss_none[r] = mine;
-    loss = mine;
+    if (reduction == FLB200_REDUCE_NONE) loss[r] = mine;
+    all.loss = mine;
   }
-  loss = warp_sum(loss);
-  n = warp_sum(n);
-  if (lane == 0) sums[blockIdx.x] = make_double2(loss, n);
+  all = sum_of_warp(all);
+  if (lane == 0) {
+    if (gridDim.x == 1) write_loss(all, reduction, loss, count, bad);
+    else sums[blockIdx.x] = all;
+  }
 }
-__global__ void __launch_bounds__(256)
-finish_loss_kernel(const double2* __restrict__ sums, int n, float* __restrict__ loss, int32_t* __restrict__ count,
-                   int reduction) {
+__global__ void __launch_bounds__(32)
+finish_loss_kernel(const LossSums* __restrict__ sums, int n, int reduction, float* __restrict__ loss,
+                   int32_t* __restrict__ count, int32_t* __restrict__ bad) {
   chain_begin();
-  __shared__ double scratch[32];
-  double s = 0.0, c = 0.0;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    s += sums[i].x;
-    c += sums[i].y;
+  LossSums all{0.0, 0, 0};
+  for (int i = threadIdx.x; i < n; i += 32) {
+    const LossSums x = sums[i];
+    all.loss += x.loss;
+    all.count += x.count;
+    all.bad |= x.bad;
   }
-  s = block_sum(s, scratch);
-  c = block_sum(c, scratch);
-  if (threadIdx.x == 0) {
-    if (count) *count = (int32_t)(c + 0.5);
-    if (reduction == FLB200_REDUCE_MEAN) loss[0] = (float)(s / c);
-    else if (reduction == FLB200_REDUCE_SUM) loss[0] = (float)s;
-  }
+  all = sum_of_warp(all);
+  if (threadIdx.x == 0) write_loss(all, reduction, loss, count, bad);
 }
 
 // Each row's RowInfo, its weight step * g_r / max |g|, zero where the row does not count; factor = max |g| / step
@@ -538,14 +567,14 @@ struct Carve {
 struct ForwardScratch {
   float2* partial;
   float* target_score;
-  double2* sums;
+  LossSums* sums;
   uint16_t *x, *w;
   ForwardScratch(Carve& c, const Shape& s) {
     // parts: two per 256 or 128 columns or one per 64, and a short one per piece
     const long long pieces = (s.classes + s.piece - 1) / s.piece;
     partial = c.take<float2>(((s.classes + 63) / 64 + 2 * pieces) * s.rows);
     target_score = c.take<float>(s.rows);
-    sums = c.take<double2>((s.rows + 31) / 32);
+    sums = c.take<LossSums>((s.rows + 31) / 32);
     x = c.take<uint16_t>(s.copy_x ? s.rows * s.x_ld : 0);
     w = c.take<uint16_t>(s.copy_w ? s.dim * s.w_ld : 0);
   }
@@ -680,10 +709,12 @@ int flb200_linear_cce_forward(const flb200_linear_cce_desc* d, const void* x, co
   }
   const int blocks = (int)((s.rows + 31) / 32);
   launch_chained(join_lse_kernel, blocks, 32 * kJoin, 0, st, scratch.partial, parts, scratch.target_score, targets,
-                 d->ignore_index, s.classes, (int)s.rows, lse,
-                 d->reduction == FLB200_REDUCE_NONE ? loss : nullptr, scratch.sums, bad_target_flag);
+                 d->ignore_index, s.classes, (int)s.rows, d->reduction, lse, loss, count_out, bad_target_flag,
+                 scratch.sums);
   FLB200_AFTER_LAUNCH("linear_cce_join");
-  launch_chained(finish_loss_kernel, 1, 256, 0, st, scratch.sums, blocks, loss, count_out, d->reduction);
+  if (blocks == 1) return FLB200_OK;
+  launch_chained(finish_loss_kernel, 1, 32, 0, st, scratch.sums, blocks, d->reduction, loss, count_out,
+                 bad_target_flag);
   FLB200_AFTER_LAUNCH("linear_cce_loss");
   return FLB200_OK;
 }
@@ -705,6 +736,7 @@ int flb200_linear_cce_backward(const flb200_linear_cce_desc* d, const void* x, c
   Carve carve{static_cast<char*>(workspace)};
   const BackwardScratch scratch(carve, s, true, true);
   const bool bf16 = d->dtype == FLB200_BF16;
+  const bool at_once = s.piece >= s.classes && scratch.dx_splits == 1;  // one product makes dx
   launch_chained(row_weights_kernel, 1, 1024, 0, st, grad_loss, targets, count, lse, d->reduction, d->ignore_index,
                  s.classes, (int)s.rows, bf16 ? 1.f : 32768.f, scratch.rows, scratch.factor);
   FLB200_AFTER_LAUNCH("linear_cce_weights");
@@ -737,15 +769,13 @@ int flb200_linear_cce_backward(const flb200_linear_cce_desc* d, const void* x, c
       if (int rc = matrix_operand(false, s.piece, scratch.grad, s.rows, cols, kBM, s.operand, &q.ma, &q.pa)) return rc;
       if (int rc = matrix_operand(false, s.w_ld, o.w, s.dim, cols, q.plan.b_box_rows(), s.operand, &q.mb, &q.pb))
         return rc;
-      const auto sums = [&](auto& g) {
-        g.out = scratch.dx;
-        g.ld = s.dim;
-        g.split_stride = s.rows * s.dim;
-        g.factor = nullptr;
-        g.vec = s.dim % 4 == 0;
-      };
-      if (int rc = col0 == 0 ? launch_product<SumFirst>("linear_cce_dx", q, sums, st)
-                             : launch_product<SumNext>("linear_cce_dx", q, sums, st))
+      const bool vec = s.dim % 4 == 0;
+      const auto sums = [&](auto& g) { g.set(scratch.dx, s.dim, s.rows * s.dim, nullptr, vec); };
+      const auto result = [&](auto& g) { g.set(grad_x, s.dim, 0, scratch.factor, vec && aligned16(grad_x)); };
+      if (int rc = at_once    ? (bf16 ? launch_product<Result16<__nv_bfloat16>::Of>("linear_cce_dx", q, result, st)
+                                      : launch_product<Result16<__half>::Of>("linear_cce_dx", q, result, st))
+                   : col0 == 0 ? launch_product<SumFirst>("linear_cce_dx", q, sums, st)
+                               : launch_product<SumNext>("linear_cce_dx", q, sums, st))
         return rc;
     }
     if (grad_w) {
@@ -757,17 +787,15 @@ int flb200_linear_cce_backward(const flb200_linear_cce_desc* d, const void* x, c
       if (int rc = matrix_operand(true, s.piece, scratch.grad, cols, s.rows, q.plan.b_box_rows(), s.operand, &q.mb,
                                   &q.pb))
         return rc;
+      const long long bytes = grad_w_dtype == FLB200_F32 ? 4 : 2;
       const auto result = [&](auto& g) {
-        using T = std::remove_reference_t<decltype(*g.out)>;
-        g.out = static_cast<T*>(grad_w) + col0;
-        g.ld = s.classes;
-        g.split_stride = 0;
-        g.factor = scratch.factor;
-        g.vec = s.classes % 4 == 0 && aligned16(grad_w);
+        g.set(static_cast<char*>(grad_w) + col0 * bytes, s.classes, 0, scratch.factor,
+              s.classes % 4 == 0 && aligned16(grad_w));
       };
-      if (int rc = grad_w_dtype == FLB200_F32 ? launch_product<SumFirst>("linear_cce_dw", q, result, st)
-                   : bf16                     ? launch_product<WeightBf16>("linear_cce_dw", q, result, st)
-                                              : launch_product<WeightF16>("linear_cce_dw", q, result, st))
+      if (int rc = grad_w_dtype == FLB200_F32
+                       ? launch_product<SumFirst>("linear_cce_dw", q, result, st)
+                       : (bf16 ? launch_product<Result16<__nv_bfloat16>::Of>("linear_cce_dw", q, result, st)
+                               : launch_product<Result16<__half>::Of>("linear_cce_dw", q, result, st)))
         return rc;
     }
     if (grad_bias) {
@@ -776,7 +804,7 @@ int flb200_linear_cce_backward(const flb200_linear_cce_desc* d, const void* x, c
       FLB200_AFTER_LAUNCH("linear_cce_dbias");
     }
   }
-  if (grad_x) {
+  if (grad_x && !at_once) {
     const long long n = s.rows * s.dim;
     const int vec = n % 4 == 0 && aligned16(grad_x);
     if (bf16)

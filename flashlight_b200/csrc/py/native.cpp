@@ -1083,12 +1083,9 @@ NATIVE(linear_cce_forward) {
   Tensor loss = floats(d.reduction == FLB200_REDUCE_NONE ? d.rows : 1, in), lse = floats(d.rows, in);
   Tensor meta = empty({2}, ScalarType::Int, in);  // [count, bad-target flag]
   int32_t* m = static_cast<int32_t*>(meta.data_ptr());
-  void* st = stream();
-  if (unlocked(cudaMemsetAsync, m, 0, (size_t)8, static_cast<cudaStream_t>(st)) != cudaSuccess)
-    check(FLB200_LAUNCH_FAILURE);
   Workspace ws(flb200_linear_cce_workspace_bytes(&d, P(in), P(w), 0), in);
   check(unlocked(flb200_linear_cce_forward, &d, P(in), P(w), Pf(bias), static_cast<const int32_t*>(P(tg)), Pf(&loss),
-                 Pf(&lse), m, m + 1, ws.p(), ws.bytes, st));
+                 Pf(&lse), m, m + 1, ws.p(), ws.bytes, stream()));
   return wrap({loss, meta, lse});
 }
 // (x, weight, bias or None, lse, grad_loss, targets, meta, reduction, ignore_index, need_x, need_w, need_b, wide)
