@@ -284,6 +284,7 @@ struct Product {  // D[M][N] over K, 16-bit operands
   long long M, N, K;
   Launch plan;
   int operand;
+  int n_fast = 0;  // pair tiles of one pair of row tiles behind one another: for a large row operand and few columns
   CUtensorMap ma, mb;
   OperandPlan pa, pb;
 };
@@ -312,7 +313,7 @@ int launch_as(const char* name, const Product& p, const Fill& fill, cudaStream_t
   g.tiles_m = (int)((p.M + kBM - 1) / kBM);
   g.tiles_n = (int)((p.N + BN - 1) / BN);
   g.Z = 1;
-  g.pair_n_fast = 0;
+  g.pair_n_fast = p.n_fast;
   fill(g);
   if constexpr (BN == 256) {
     if (p.plan.pairs)
@@ -763,6 +764,7 @@ int flb200_linear_cce_backward(const flb200_linear_cce_desc* d, const void* x, c
       Product q;
       q.M = s.rows; q.N = s.dim; q.K = cols;
       q.operand = s.operand;
+      q.n_fast = 1;  // (G once from memory: 4096 x 768 of 16384 columns read 295 MB without)
       q.plan = plan_dx(s, std::min(s.piece, s.classes));
       // (a last, short piece may have fewer splits: it adds to the sums of the first of them)
       q.plan.splits = fit_splits(cols, scratch.dx_splits, &q.plan.iters_per_split);
