@@ -21,7 +21,6 @@
 #include <type_traits>
 
 #include "common.cuh"
-#include "packed.cuh"
 
 namespace flb200 {
 namespace {
@@ -109,15 +108,21 @@ __device__ __forceinline__ void store8(T* p, bool whole, int live, const float* 
   }
 }
 
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // 8-bit states: the values of eight codes over their block's scale
 __device__ __forceinline__ void widen_codes(const Eight<uint8_t>& r, float scale, float* v) {
-  const F2 s = pair(scale);
 #pragma unroll
   for (int j = 0; j < kPer; j += 2) {
     const __half2_raw h =
         __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(r.w[j >> 2] >> (8 * (j & 2))), __NV_E4M3);
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    unpair(pair(f.x, f.y) * s, v[j], v[j + 1]);
+    v[j] = f.x * scale;
+    v[j + 1] = f.y * scale;
   }
 }
 __device__ __forceinline__ Eight<uint8_t> codes_live(const uint8_t* p, int live) {
@@ -139,12 +144,10 @@ __device__ __forceinline__ void store_codes(uint8_t* p, float* scale, bool whole
   for (int j = 0; j < kPer; ++j) top = fmaxf(top, kRoot ? v[j] : fabsf(v[j]));  // (past the end: zeros)
   top = fmaxf(warp_top(top), 1e-30f);
   const float to_code = __fmul_rn(__frcp_rn(top), 448.f);
-  const F2 k = pair(to_code);
   uint32_t w[2] = {0, 0};
 #pragma unroll
   for (int j = 0; j < kPer; j += 2) {
-    float2 s;
-    unpair(pair(v[j], v[j + 1]) * k, s.x, s.y);
+    float2 s = make_float2(v[j] * to_code, v[j + 1] * to_code);
     if (kRoot) {
       if (v[j] > 0.f) s.x = fmaxf(s.x, 0x1p-9f);
       if (v[j + 1] > 0.f) s.y = fmaxf(s.y, 0x1p-9f);
@@ -264,23 +267,15 @@ adamw_kernel(const __grid_constant__ AdamwTable<CAP> table, const AdamwMath k) {
     // Each operation of the moments rounds by itself (no contraction): what is kept in 8 bits then depends on
     // the formula alone.
 #pragma unroll
-    for (int j = 0; j < kPer; j += 2) {
-      const F2 gg = pair(g[j], g[j + 1]) * pair(k.grad_scale);
-      const F2 mm = add_apart(pair(m[j], m[j + 1]) * pair(k.beta1), gg * pair(k.rest1));
-      F2 vv = pair(v[j], v[j + 1]);
-      if (BITS == 8) vv = vv * vv;
-      vv = add_apart(vv * pair(k.beta2), gg * gg * pair(k.rest2));
-      float v0, v1, d0, d1, u0, u1;
-      unpair(vv, v0, v1);
-      const float r0 = __fsqrt_rn(v0), r1 = __fsqrt_rn(v1);
-      unpair(fused(pair(r0, r1), pair(k.inv_root_c2), pair(k.epsilon)), d0, d1);
-      unpair(mm * pair(k.inv_c1), u0, u1);
-      const F2 pp = pair(p[j], p[j + 1]);
-      const F2 step = fused(pp, pair(k.weight_decay), pair(__fdividef(u0, d0), __fdividef(u1, d1)));
-      unpair(fused(step, pair(-k.lr), pp), p[j], p[j + 1]);
-      unpair(mm, m[j], m[j + 1]);
-      v[j] = BITS == 32 ? v0 : r0;
-      v[j + 1] = BITS == 32 ? v1 : r1;
+    for (int j = 0; j < kPer; ++j) {
+      const float gg = __fmul_rn(g[j], k.grad_scale);
+      m[j] = __fadd_rn(__fmul_rn(m[j], k.beta1), __fmul_rn(gg, k.rest1));
+      const float old = BITS == 8 ? __fmul_rn(v[j], v[j]) : v[j];
+      const float vv = __fadd_rn(__fmul_rn(old, k.beta2), __fmul_rn(__fmul_rn(gg, gg), k.rest2));
+      const float root = __fsqrt_rn(vv);
+      const float step = m[j] * k.inv_c1 * reciprocal(fmaf(root, k.inv_root_c2, k.epsilon));
+      p[j] = fmaf(-k.lr, fmaf(k.weight_decay, p[j], step), p[j]);
+      v[j] = BITS == 32 ? vv : root;
     }
     store8(static_cast<TP*>(t.param) + i, whole, live, p);
     if constexpr (BITS == 32) {

@@ -315,12 +315,13 @@ int launch_as(const char* name, const Product& p, const Fill& fill, cudaStream_t
   g.Z = 1;
   g.pair_n_fast = p.n_fast;
   fill(g);
+  const long long tiles = (long long)g.tiles_m * g.tiles_n * g.splits;
+  FLB200_REQUIRE(tiles < 0x7fffffffLL, "%s: too many tiles", name);
   if constexpr (BN == 256) {
     if (p.plan.pairs)
       return launch_pair_problem<Problem<BN>, BN>(name, p.ma, p.mb, g,
                                                   (long long)((g.tiles_m + 1) / 2) * g.tiles_n * g.splits, st);
   }
-  const long long tiles = (long long)g.tiles_m * g.tiles_n * g.splits;
   constexpr int kSub = BN <= 128 ? 2 : 1;
   return launch_problem_as<Problem<BN>, BN, stages_for(BN), 0, kSub>(name, p.ma, p.mb, g, tiles, st);
 }
@@ -461,7 +462,7 @@ row_weights_kernel(const float* __restrict__ grad_loss, const int32_t* __restric
   chain_begin();
   __shared__ float scratch[32];
   float top = 0.f;
-  if (reduction == FLB200_REDUCE_NONE) {
+  if (reduction == FLB200_REDUCE_NONE) {  // (one CTA)
     for (int r = threadIdx.x; r < rows; r += 1024)
       if (counts(targets[r], ignore, classes)) top = fmaxf(top, fabsf(grad_loss[r]));
     top = warp_max(top);
@@ -472,8 +473,8 @@ row_weights_kernel(const float* __restrict__ grad_loss, const int32_t* __restric
     top = grad_loss[0];
     if (reduction == FLB200_REDUCE_MEAN) top = *count > 0 ? top / (float)*count : 0.f;
   }
-  if (threadIdx.x == 0) *factor = top / step;
-  for (int r = threadIdx.x; r < rows; r += 1024) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *factor = top / step;
+  for (int r = blockIdx.x * 1024 + threadIdx.x; r < rows; r += gridDim.x * 1024) {
     float w = 0.f;
     if (counts(targets[r], ignore, classes))
       w = reduction != FLB200_REDUCE_NONE ? step : (top > 0.f ? step * (grad_loss[r] / top) : 0.f);
@@ -738,7 +739,8 @@ int flb200_linear_cce_backward(const flb200_linear_cce_desc* d, const void* x, c
   const BackwardScratch scratch(carve, s, true, true);
   const bool bf16 = d->dtype == FLB200_BF16;
   const bool at_once = s.piece >= s.classes && scratch.dx_splits == 1;  // one product makes dx
-  launch_chained(row_weights_kernel, 1, 1024, 0, st, grad_loss, targets, count, lse, d->reduction, d->ignore_index,
+  const unsigned row_ctas = d->reduction == FLB200_REDUCE_NONE ? 1u : (unsigned)((s.rows + 1023) / 1024);
+  launch_chained(row_weights_kernel, row_ctas, 1024, 0, st, grad_loss, targets, count, lse, d->reduction, d->ignore_index,
                  s.classes, (int)s.rows, bf16 ? 1.f : 32768.f, scratch.rows, scratch.factor);
   FLB200_AFTER_LAUNCH("linear_cce_weights");
   for (long long col0 = 0; col0 < s.classes; col0 += s.piece) {

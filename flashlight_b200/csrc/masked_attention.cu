@@ -1127,7 +1127,8 @@ int check_attention(const char* name, const flb200_attention_desc* d) {
                      d->heads % d->kv_heads == 0 && d->head_dim >= 1,
                  "%s: bad extents", name);
   FLB200_REQUIRE(d->scale > 0.f && d->scale < 1e30f, "%s: the scale must be positive", name);
-  FLB200_REQUIRE(d->softcap >= 0.f && d->softcap < 1e30f, "%s: the cap must be positive, or 0 for none", name);
+  FLB200_REQUIRE(d->softcap >= 0.f && d->softcap < 1e30f && (d->softcap == 0.f || d->scale / d->softcap < 1e30f),
+                 "%s: the cap must be positive, or 0 for none", name);
   if (!flb200_masked_attention_supported(d))
     return fail(FLB200_UNSUPPORTED, "%s: built for f16 and bf16 and head dimensions that are multiples of 8 up to 128",
                 name);

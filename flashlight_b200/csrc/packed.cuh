@@ -31,12 +31,4 @@ __device__ __forceinline__ F2 fused(F2 a, F2 b, F2 c) {  // a b + c
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x.r) : "l"(a.r), "l"(b.r), "l"(c.r));
   return x;
 }
-// a + b, one by one: the assembler makes one rounding of a paired product and a paired sum behind it.
-__device__ __forceinline__ F2 add_apart(F2 a, F2 b) {
-  float a0, a1, b0, b1;
-  unpair(a, a0, a1);
-  unpair(b, b0, b1);
-  return pair(__fadd_rn(a0, b0), __fadd_rn(a1, b1));
-}
-
 }  // namespace flb200
