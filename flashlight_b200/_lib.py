@@ -76,7 +76,7 @@ class LinearCceDesc(C.Structure):
 
 class AttentionDesc(C.Structure):
     _fields_ = [(n, i64) for n in ("batch", "q_len", "k_len", "heads", "kv_heads", "head_dim")] + [
-        ("scale", f32), ("softcap", f32), ("dtype", i32)]
+        ("scale", f32), ("softcap", f32), ("dtype", i32), ("causal", i32), ("prefix", vp)]
 
 
 class HeadTensor(C.Structure):

@@ -6,7 +6,8 @@
 //     dq = scale dS k    dk = scale dS^T q    dv = P^T do           (dk, dv summed over the heads that share them)
 // flashlight/fl/autograd/Functions.cpp:1828-1891 is the chain of whole-tensor operators for this, its mask an
 // additive tensor.  One interval per query says all that a causal mask, documents packed into a row, a prefix and
-// padding say together; flb200_attention_mask makes it once per batch, with what the kernels below need to know
+// padding say together.  Without documents it is a formula; with them flb200_attention_mask makes a table of it once per
+// batch, with what the kernels below need to know
 // of blocks of 128: which key blocks a query block meets, and whether all of a block is seen.
 //
 // The scores of a 128 x 128 block live in tensor memory only.  tanh(u) = 1 - 2 r, r = 1 / (1 + e^2u), from the
@@ -41,12 +42,36 @@ constexpr int kFwdThreads = 320;   // warps 0..7: two threads per row; 8: TMA; 9
 // rows: [lo, hi) of each query ([batch][q_len]; hi <= lo: it sees nothing).  q_blocks: of each block of queries the
 // least lo and the greatest hi of those that see something, and the greatest lo and the least hi of all (an
 // empty row makes that pair empty).  k_blocks: the query blocks [first, last) that may see a block of keys.
+__host__ __device__ inline int blocks_of(long long n) { return (int)((n + kBlock - 1) / kBlock); }
 struct MaskView {
-  const int2* rows;
+  const int2* rows;  // null: no documents, what follows is computed
   const int4* q_blocks;
   const int2* k_blocks;
+  const int* prefix;
+  int causal, q_len, k_len;
+
+  __device__ __forceinline__ int seen_by_all(int batch) const {
+    return prefix ? min(max(prefix[batch], 0), k_len) : 0;
+  }
+  __device__ __forceinline__ int end_of(int i, int all) const {  // of row i's interval, without documents
+    return causal ? max(i + k_len - q_len + 1, all) : k_len;
+  }
+  __device__ __forceinline__ int2 row(int batch, int i) const {
+    if (rows) return rows[(long long)batch * q_len + i];
+    return make_int2(0, end_of(i, seen_by_all(batch)));
+  }
+  __device__ __forceinline__ int4 q_block(int batch, int b) const {
+    if (rows) return q_blocks[(long long)batch * blocks_of(q_len) + b];
+    const int all = seen_by_all(batch);
+    return make_int4(0, end_of(min(q_len, (b + 1) * kBlock) - 1, all), 0, end_of(b * kBlock, all));
+  }
+  __device__ __forceinline__ int2 k_block(int batch, int j) const {
+    if (rows) return k_blocks[(long long)batch * blocks_of(k_len) + j];
+    // the first block with a query at or behind the block's first key; all where the prefix reaches into it
+    const int behind = j * kBlock - (k_len - q_len);
+    return make_int2(causal && behind > 0 && seen_by_all(batch) <= j * kBlock ? behind / kBlock : 0, blocks_of(q_len));
+  }
 };
-__host__ __device__ inline int blocks_of(long long n) { return (int)((n + kBlock - 1) / kBlock); }
 inline size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 size_t mask_bytes(long long batch, long long q_len, long long k_len) {
   return round16(batch * blocks_of(q_len) * sizeof(int4)) + round16(batch * blocks_of(k_len) * sizeof(int2)) +
@@ -54,7 +79,10 @@ size_t mask_bytes(long long batch, long long q_len, long long k_len) {
 }
 MaskView mask_view(const void* mask, long long batch, long long q_len, long long k_len) {
   const char* p = static_cast<const char*>(mask);
-  MaskView v;
+  MaskView v{};
+  v.q_len = (int)q_len;
+  v.k_len = (int)k_len;
+  if (!mask) return v;
   v.q_blocks = reinterpret_cast<const int4*>(p);
   p += round16(batch * blocks_of(q_len) * sizeof(int4));
   v.k_blocks = reinterpret_cast<const int2*>(p);
@@ -63,22 +91,27 @@ MaskView mask_view(const void* mask, long long batch, long long q_len, long long
   return v;
 }
 
-// Inclusive running maximum over the CTA's 1024 threads, in thread order, of a carry and each thread's value.
-__device__ __forceinline__ int running_max(int v, int carry, int* scratch, int* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ int warp_running_max(int v) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v = max(v, u);
   }
+  return v;
+}
+// Of the CTA's 1024 threads, the maximum of `carry` and the values of those before this one; carry becomes that of all.
+__device__ __forceinline__ int max_before(int v, int* carry, int* scratch) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  v = warp_running_max(v);
   __syncthreads();  // scratch may still be read from the call before
   if (lane == 31) scratch[warp] = v;
   __syncthreads();
-  int before = carry;
-  for (int w = 0; w < warp; ++w) before = max(before, scratch[w]);
-  *total = carry;
-  for (int w = 0; w < 32; ++w) *total = max(*total, scratch[w]);
-  return max(v, before);
+  const int warps = max(warp_running_max(scratch[lane]), *carry);
+  const int ahead = __shfl_sync(0xffffffffu, warps, (warp + 31) & 31), mine = __shfl_up_sync(0xffffffffu, v, 1);
+  const int before = warp > 0 ? ahead : *carry;
+  *carry = __shfl_sync(0xffffffffu, warps, 31);
+  return lane > 0 ? max(before, mine) : before;
 }
 
 // One CTA per row of the batch: a query's document is the run of equal ids around its position, and the ends of the
@@ -91,72 +124,54 @@ attention_mask_kernel(const int* __restrict__ documents, const int* __restrict__
   __shared__ int scratch[32];
   const int b = blockIdx.x, off = k_len - q_len, step = 1024 * kRun;
   const int nq = blocks_of(q_len), nk = blocks_of(k_len);
-  const int* ids = documents ? documents + (long long)b * k_len : nullptr;
+  const int* ids = documents + (long long)b * k_len;
   const int seen_by_all = prefix ? min(max(prefix[b], 0), k_len) : 0;
   rows += (long long)b * q_len;
   q_blocks += (long long)b * nq;
   k_blocks += (long long)b * nk;
-  if (!ids) {
-    for (int i = threadIdx.x; i < q_len; i += 1024)
-      rows[i] = make_int2(0, causal ? max(i + off + 1, seen_by_all) : k_len);
-  } else {
-    int carry = 0;
-    for (int p0 = 0; p0 < k_len; p0 += step) {
-      int start[kRun], id[kRun], last = 0;
-      const int p = p0 + threadIdx.x * kRun;
-      int before = p > 0 && p < k_len ? ids[p - 1] : 0;
+  int carry = 0;
+  for (int p0 = 0; p0 < k_len; p0 += step) {
+    int start[kRun], id[kRun], last = 0;
+    const int p = p0 + threadIdx.x * kRun;
+    int before = p > 0 && p < k_len ? ids[p - 1] : 0;
 #pragma unroll
-      for (int j = 0; j < kRun; ++j) {
-        id[j] = p + j < k_len ? ids[p + j] : 0;
-        if (p + j < k_len && (p + j == 0 || id[j] != before)) last = p + j;
-        start[j] = last;
-        before = id[j];
-      }
-      int total;
-      // (of the threads before; this one's own runs come on top)
-      const int through = running_max(last, carry, scratch, &total);
-      const int mine = __shfl_up_sync(0xffffffffu, through, 1);
-      int left = carry;
-      if ((threadIdx.x & 31) > 0) left = mine;
-      else for (int w = 0; w < (int)(threadIdx.x >> 5); ++w) left = max(left, scratch[w]);
-      carry = total;
-#pragma unroll
-      for (int j = 0; j < kRun; ++j) {
-        const int i = p + j - off;
-        if (p + j < k_len && i >= 0)
-          rows[i] = id[j] < 0 ? make_int2(0, 0)
-                              : make_int2(max(start[j], left), causal ? p + j + 1 : k_len);
-      }
+    for (int j = 0; j < kRun; ++j) {
+      id[j] = p + j < k_len ? ids[p + j] : 0;
+      if (p + j < k_len && (p + j == 0 || id[j] != before)) last = p + j;
+      start[j] = last;
+      before = id[j];
     }
-    if (!causal || seen_by_all > 0) {  // the runs' ends count
-      int from_right = 0;  // k_len - end, running
-      const int last0 = (k_len - 1) / step * step;
-      for (int p0 = last0; p0 >= 0; p0 -= step) {
-        // thread t looks at positions from the right: the chunk's last kRun positions are thread 0's
-        const int p = p0 + step - 1 - threadIdx.x * kRun;
-        int end[kRun], id[kRun], last = 0;
-        int behind = p + 1 < k_len ? ids[p + 1] : 0;
+    const int left = max_before(last, &carry, scratch);
 #pragma unroll
-        for (int j = 0; j < kRun; ++j) {
-          id[j] = p - j < k_len ? ids[p - j] : 0;
-          if (p - j < k_len && p - j + 1 < k_len && id[j] != behind) last = k_len - (p - j + 1);
-          end[j] = last;
-          behind = id[j];
-        }
-        int total;
-        const int through = running_max(last, from_right, scratch, &total);
-        const int mine = __shfl_up_sync(0xffffffffu, through, 1);
-        int right = from_right;
-        if ((threadIdx.x & 31) > 0) right = mine;
-        else for (int w = 0; w < (int)(threadIdx.x >> 5); ++w) right = max(right, scratch[w]);
-        from_right = total;
+    for (int j = 0; j < kRun; ++j) {
+      const int i = p + j - off;
+      if (p + j < k_len && i >= 0)
+        rows[i] = id[j] < 0 ? make_int2(0, 0)
+                            : make_int2(max(start[j], left), causal ? p + j + 1 : k_len);
+    }
+  }
+  if (!causal || seen_by_all > 0) {  // the runs' ends count
+    int from_right = 0;  // k_len - end, running
+    const int last0 = (k_len - 1) / step * step;
+    for (int p0 = last0; p0 >= 0; p0 -= step) {
+      // thread t looks at positions from the right: the chunk's last kRun positions are thread 0's
+      const int p = p0 + step - 1 - threadIdx.x * kRun;
+      int end[kRun], id[kRun], last = 0;
+      int behind = p + 1 < k_len ? ids[p + 1] : 0;
 #pragma unroll
-        for (int j = 0; j < kRun; ++j) {
-          const int i = p - j - off;
-          if (p - j < k_len && i >= 0 && id[j] >= 0) {
-            const int e = k_len - max(end[j], right);
-            rows[i].y = causal ? min(e, max(p - j + 1, seen_by_all)) : e;
-          }
+      for (int j = 0; j < kRun; ++j) {
+        id[j] = p - j < k_len ? ids[p - j] : 0;
+        if (p - j < k_len && p - j + 1 < k_len && id[j] != behind) last = k_len - (p - j + 1);
+        end[j] = last;
+        behind = id[j];
+      }
+      const int right = max_before(last, &from_right, scratch);
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        const int i = p - j - off;
+        if (p - j < k_len && i >= 0 && id[j] >= 0) {
+          const int e = k_len - max(end[j], right);
+          rows[i].y = causal ? min(e, max(p - j + 1, seen_by_all)) : e;
         }
       }
     }
@@ -438,7 +453,7 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   const int all_heads = gridDim.x / nq;
   const int i = nq - 1 - (int)blockIdx.x / all_heads;  // of all heads the longest of a causal mask first
   const int bh = blockIdx.x % all_heads, batch = bh / a.s.heads, head = bh - batch * a.s.heads;
-  const int4 info = a.s.mask.q_blocks[(long long)batch * nq + i];
+  const int4 info = a.s.mask.q_block(batch, i);
   const int begin = info.y > info.x ? info.x / kBlock : 0;
   const int blocks = info.y > info.x ? blocks_of(info.y) - begin : 0;
 
@@ -536,7 +551,7 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     const uint32_t s_addr = lane_addr + 64u * half, p_addr = lane_addr + kP + 32u * half;
     const uint32_t o_addr = lane_addr + 128u + (uint32_t)(D / 2 * half);
     int2 seen = make_int2(0, 0);
-    if (q < a.s.q_len) seen = a.s.mask.rows[(long long)batch * a.s.q_len + q];
+    if (q < a.s.q_len) seen = a.s.mask.row(batch, q);
     const float slope = BIAS ? a.s.slopes[head] * kLog2e : 0.f;
     float ref = -1e30f, sum = 0.f;  // in powers of 2; a row that has seen nothing yet is far below all scores
     float lost = 0.f;               // of the largest P, by rounding
@@ -764,12 +779,12 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
   int first, count, total;  // column blocks, and how many there are over all heads
   int4 info = make_int4(0, 0, 0, 0);
   if (KV) {
-    const int2 r = a.s.mask.k_blocks[(long long)batch * nk + block];
+    const int2 r = a.s.mask.k_block(batch, block);
     first = r.x;
     count = max(r.y - r.x, 0);
     total = count * a.s.group;
   } else {
-    info = a.s.mask.q_blocks[(long long)batch * nq + block];
+    info = a.s.mask.q_block(batch, block);
     first = info.y > info.x ? info.x / kBlock : 0;
     count = info.y > info.x ? blocks_of(info.y) - first : 0;
     total = count;
@@ -882,7 +897,7 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
     if (!KV && mine < a.s.q_len) {
       my_lse = lse_of(rows0 + mine);
       my_d = a.dsum[rows0 + mine];
-      seen = a.s.mask.rows[(long long)batch * a.s.q_len + mine];
+      seen = a.s.mask.row(batch, mine);
     }
     if (BIAS && !KV) slope = a.s.slopes[head] * kLog2e;
     // of a unit's columns, where they are queries: lse, D and the interval, a thread per column
@@ -892,7 +907,7 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
       const int q = (first + in_head) * kBlock + 64 * (u & 1) + tid;
       if (tid < 64 && q < a.s.q_len) {
         const long long at = rows0 + (long long)hq * a.s.q_len + q;
-        c.seen = a.s.mask.rows[(long long)batch * a.s.q_len + q];
+        c.seen = a.s.mask.row(batch, q);
         c.ld = make_float2(lse_of(at), a.dsum[at]);
       }
       return c;
@@ -921,7 +936,7 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
       settle_head();
       if (KV) {
         asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");  // the columns are there
-        const int4 q = a.s.mask.q_blocks[(long long)batch * nq + first + this_in];
+        const int4 q = a.s.mask.q_block(batch, first + this_in);
         whole = q.z <= block * kBlock && q.w >= (block + 1) * kBlock;
         if (BIAS) slope = a.s.slopes[head * a.s.group + this_hq] * kLog2e;
         if (u + kUnits < 2 * total) ahead = column(u + kUnits, in_head, hq);
@@ -1113,6 +1128,8 @@ AttnShape shape_of(const flb200_attention_desc* d, const float* slopes, const vo
   s.group = (int)(d->heads / d->kv_heads);
   s.head_dim = (int)d->head_dim;
   s.mask = mask_view(mask, d->batch, d->q_len, d->k_len);
+  s.mask.causal = d->causal ? 1 : 0;
+  s.mask.prefix = mask ? nullptr : d->prefix;
   s.slopes = slopes;
   s.scale = d->scale;
   s.to_log2 = d->scale * kLog2e;
@@ -1126,6 +1143,7 @@ int check_attention(const char* name, const flb200_attention_desc* d) {
   FLB200_REQUIRE(d->batch >= 1 && d->q_len >= 1 && d->k_len >= d->q_len && d->heads >= 1 && d->kv_heads >= 1 &&
                      d->heads % d->kv_heads == 0 && d->head_dim >= 1,
                  "%s: bad extents", name);
+  FLB200_REQUIRE(d->causal || !d->prefix, "%s: a prefix belongs to a causal mask", name);
   FLB200_REQUIRE(d->scale > 0.f && d->scale < 1e30f, "%s: the scale must be positive", name);
   FLB200_REQUIRE(d->softcap >= 0.f && d->softcap < 1e30f && (d->softcap == 0.f || d->scale / d->softcap < 1e30f),
                  "%s: the cap must be positive, or 0 for none", name);
@@ -1210,6 +1228,7 @@ int flb200_attention_mask(int64_t batch, int64_t q_len, int64_t k_len, int causa
                           const int32_t* prefix, void* mask, void* stream) {
   FLB200_REQUIRE(batch >= 1 && q_len >= 1 && k_len >= q_len && k_len < (1 << 24) && batch < 65536,
                  "attention_mask: bad extents");
+  FLB200_REQUIRE(documents, "attention_mask: null documents");
   FLB200_REQUIRE(mask && aligned16(mask), "attention_mask: the mask must be 16-byte aligned");
   FLB200_REQUIRE(causal || !prefix, "attention_mask: a prefix belongs to a causal mask");
   const MaskView v = mask_view(mask, batch, q_len, k_len);
@@ -1233,7 +1252,7 @@ int flb200_masked_attention_forward(const flb200_attention_desc* d, const flb200
                                     const void* mask, const flb200_head_tensor* out, void* rest, float* lse,
                                     void* stream) {
   if (int rc = check_attention("masked_attention_forward", d)) return rc;
-  FLB200_REQUIRE(mask, "masked_attention_forward: null mask");
+  FLB200_REQUIRE(!mask || aligned16(mask), "masked_attention_forward: the mask must be 16-byte aligned");
   FLB200_REQUIRE(!rest || aligned16(rest), "masked_attention_forward: rest must be 16-byte aligned");
   for (const flb200_head_tensor* t : {q, k, v, out})
     if (int rc = check_tensor("masked_attention_forward", t)) return rc;
@@ -1267,7 +1286,8 @@ int flb200_masked_attention_backward(const flb200_attention_desc* d, const flb20
                                      const flb200_head_tensor* grad_v, void* workspace, size_t workspace_bytes,
                                      void* stream) {
   if (int rc = check_attention("masked_attention_backward", d)) return rc;
-  FLB200_REQUIRE(mask && lse, "masked_attention_backward: null mask or lse");
+  FLB200_REQUIRE(lse, "masked_attention_backward: null lse");
+  FLB200_REQUIRE(!mask || aligned16(mask), "masked_attention_backward: the mask must be 16-byte aligned");
   FLB200_REQUIRE(!rest || aligned16(rest), "masked_attention_backward: rest must be 16-byte aligned");
   for (const flb200_head_tensor* t : {q, k, v, out, grad_out, grad_q, grad_k, grad_v})
     if (int rc = check_tensor("masked_attention_backward", t)) return rc;

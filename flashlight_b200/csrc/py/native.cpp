@@ -632,17 +632,14 @@ const int32_t* ints(const Tensor* t, int64_t n, const char* what) {
   }
   return static_cast<const int32_t*>(t->data_ptr());
 }
-// (batch, q_len, k_len, causal, documents or None, prefix or None, device index) -> the mask's bytes
+// (batch, q_len, k_len, causal, documents or None, prefix or None) -> the mask's bytes, or None without documents
 NATIVE(attention_mask) {
   const int64_t B = x.i(0), q = x.i(1), k = x.i(2);
   if (B < 1 || q < 1 || k < q) value_error("attention_mask: batch >= 1 and 1 <= q_len <= k_len");
   const int32_t *docs = ints(x.t(4), B * k, "documents"), *prefix = ints(x.t(5), B, "prefix");
-  Tensor m;
-  {
-    const Unlocked u;
-    m = at::detail::empty_cuda({(int64_t)flb200_attention_mask_bytes(B, q, k)}, ScalarType::Byte,
-                               at::Device(at::kCUDA, (c10::DeviceIndex)x.i(6)), std::nullopt);
-  }
+  if (prefix && !x.b(3)) value_error("attention_mask: a prefix belongs to a causal mask");
+  if (!docs) Py_RETURN_NONE;
+  Tensor m = empty({(int64_t)flb200_attention_mask_bytes(B, q, k)}, ScalarType::Byte, x.tensor(4));
   check(unlocked(flb200_attention_mask, B, q, k, x.b(3) ? 1 : 0, docs, prefix, m.data_ptr(), stream()));
   return wrap(m);
 }
@@ -677,11 +674,11 @@ struct AttentionCall {
   Heads q, k, v;
   flb200_attention_desc d = {};
   const float* slopes = nullptr;
-  const void* mask;
-  // args: q, k, v, slopes or None, mask, its (batch, q_len, k_len), scale, softcap
+  const void* mask = nullptr;
+  // args: q, k, v, slopes or None, mask or None, its (batch, q_len, k_len, causal, prefix or None), scale, softcap
   explicit AttentionCall(const Args& x) : q(x.tensor(0), "q"), k(x.tensor(1), "k"), v(x.tensor(2), "v") {
-    const Tensor &tq = x.tensor(0), &tk = x.tensor(1), &tv = x.tensor(2), &m = x.tensor(4);
-    const Tensor* s = x.t(3);
+    const Tensor &tq = x.tensor(0), &tk = x.tensor(1), &tv = x.tensor(2);
+    const Tensor *s = x.t(3), *m = x.t(4);
     if (tk.sizes() != tv.sizes() || tq.size(0) != tk.size(0) || tq.size(3) != tk.size(3) ||
         tq.scalar_type() != tk.scalar_type() || tq.scalar_type() != tv.scalar_type())
       value_error("masked_attention: q, k and v must be of one type, batch and head dim, k and v alike");
@@ -695,11 +692,17 @@ struct AttentionCall {
     d.heads = tq.size(2);
     d.kv_heads = tk.size(2);
     d.head_dim = tq.size(3);
-    d.scale = (float)x.d(8);
-    d.softcap = (float)x.d(9);
+    d.causal = x.b(8) ? 1 : 0;
+    d.prefix = ints(x.t(9), d.batch, "prefix");
+    d.scale = (float)x.d(10);
+    d.softcap = (float)x.d(11);
     d.dtype = code_of(tq);
-    if (m.get_device() != tq.get_device()) value_error("masked_attention: the mask is on another device");
-    mask = m.data_ptr();
+    if (m) {
+      if (m->get_device() != tq.get_device() ||
+          m->numel() != (int64_t)flb200_attention_mask_bytes(d.batch, d.q_len, d.k_len))
+        value_error("masked_attention: the mask is on another device or of other extents");
+      mask = m->data_ptr();
+    }
     if (s) {
       if (s->numel() != d.heads || s->scalar_type() != ScalarType::Float || !s->is_contiguous())
         value_error("masked_attention: slopes are float32, one per query head");
@@ -712,7 +715,7 @@ NATIVE(masked_attention) {  // (AttentionCall's, train) -> (out, lse, rest), the
   const flb200_attention_desc& d = c.d;
   const Tensor& q = x.tensor(0);
   Tensor out = empty({d.batch, d.q_len, d.heads, d.head_dim}, q.scalar_type(), q), lse, rest;
-  if (x.b(10)) {
+  if (x.b(12)) {
     lse = empty({d.batch, d.heads, d.q_len}, ScalarType::Float, q);
     rest = empty_like(out);
   }
@@ -727,8 +730,8 @@ NATIVE(masked_attention) {  // (AttentionCall's, train) -> (out, lse, rest), the
 NATIVE(masked_attention_backward) {
   AttentionCall c(x);
   const flb200_attention_desc& d = c.d;
-  const Tensor &out = x.tensor(10), &gy = x.tensor(12), &lse = x.tensor(13);
-  const Tensor* rest = x.t(11);
+  const Tensor &out = x.tensor(12), &gy = x.tensor(14), &lse = x.tensor(15);
+  const Tensor* rest = x.t(13);
   if (out.sizes() != x.tensor(0).sizes() || gy.sizes() != out.sizes() || gy.scalar_type() != out.scalar_type() ||
       out.scalar_type() != x.tensor(0).scalar_type())
     value_error("masked_attention: the output's gradient must be like the output");
@@ -740,7 +743,7 @@ NATIVE(masked_attention_backward) {
   Tensor grads[3];
   for (int i = 0; i < 3; ++i) {
     const Tensor& like = x.tensor(i);
-    const Tensor* given = x.t(14 + i);
+    const Tensor* given = x.t(16 + i);
     if (given && (given->sizes() != like.sizes() || given->scalar_type() != like.scalar_type() || !Heads::fits(*given)))
       value_error("masked_attention: a given gradient must be like its tensor, in aligned rows");
     grads[i] = given ? *given : empty(like.sizes(), like.scalar_type(), like);

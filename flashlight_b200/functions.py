@@ -333,22 +333,27 @@ def softmax_backward(y, grad_y, scale: float = 1.0):
 class AttentionMask:
     """Which keys each query sees, for all heads, layers and both directions (attention_mask)."""
 
-    def __init__(self, batch: int, q_len: int, k_len: int, data):
-        self.batch, self.q_len, self.k_len, self.data = batch, q_len, k_len, data
+    def __init__(self, batch: int, q_len: int, k_len: int, causal: bool, prefix, data):
+        self.batch, self.q_len, self.k_len, self.causal, self.prefix, self.data = (
+            batch, q_len, k_len, causal, prefix, data)
+
+    def _args(self):
+        return self.data, self.batch, self.q_len, self.k_len, self.causal, self.prefix
 
 
 def attention_mask(batch: int, q_len: int, k_len: Optional[int] = None, *, causal: bool = True, documents=None,
                    prefix=None, device=None) -> AttentionMask:
-    """The mask of masked_attention, made on the device in one launch (flb200_attention_mask).  Queries are the last
-    q_len of k_len positions.  documents (batch, k_len) int32: a position sees its own run of equal ids only, ids
-    below zero see nothing; prefix (batch,) int32, with causal: positions that every query sees."""
+    """The mask of masked_attention.  Queries are the last q_len of k_len positions.  documents (batch, k_len) int32: a
+    position sees its own run of equal ids only, ids below zero see nothing (one launch makes a table of it,
+    flb200_attention_mask); prefix (batch,) int32, with causal: positions that every query sees.  device: where the
+    attention runs, if it is to be checked here."""
     k_len = q_len if k_len is None else k_len
-    given = documents if documents is not None else prefix
-    device = torch.device(device if device is not None else given.device if given is not None else "cuda")
-    if device.type != "cuda":
-        raise ValueError("the B200 autograd extension needs device (CUDA) tensors")
-    index = torch.cuda.current_device() if device.index is None else device.index
-    return AttentionMask(batch, q_len, k_len, N.attention_mask(batch, q_len, k_len, causal, documents, prefix, index))
+    if device is not None:
+        for t in (documents, prefix):
+            if t is not None and t.device.type != torch.device(device).type:
+                raise ValueError(f"attention_mask: documents and prefix must be on {device}")
+    return AttentionMask(batch, q_len, k_len, causal, prefix,
+                         N.attention_mask(batch, q_len, k_len, causal, documents, prefix))
 
 
 def masked_attention(q, k, v, mask: AttentionMask, scale: float, softcap: float = 0.0, slopes=None,
@@ -357,11 +362,11 @@ def masked_attention(q, k, v, mask: AttentionMask, scale: float, softcap: float 
     kernel: q (batch, q_len, heads, head dim), k and v (batch, k_len, key heads, head dim), f16 or bf16, any strides
     (those of whole 16-byte rows are read in place).  slopes: float32 per query head, or None.  Returns (out, lse,
     rest): what the gradient needs besides, each row's log-sum-exp and what the rounding of out took, or None."""
-    return N.masked_attention(q, k, v, slopes, mask.data, mask.batch, mask.q_len, mask.k_len, scale, softcap, train)
+    return N.masked_attention(q, k, v, slopes, *mask._args(), scale, softcap, train)
 
 
 def masked_attention_backward(q, k, v, out, rest, grad_out, lse, mask: AttentionMask, scale: float,
                               softcap: float = 0.0, slopes=None, grads=(None, None, None)):
     """(grad_q, grad_k, grad_v) of masked_attention, into the tensors of `grads` where they are given."""
-    return N.masked_attention_backward(q, k, v, slopes, mask.data, mask.batch, mask.q_len, mask.k_len, scale, softcap,
+    return N.masked_attention_backward(q, k, v, slopes, *mask._args(), scale, softcap,
                                        out, rest, grad_out, lse, *grads)

@@ -341,8 +341,7 @@ class TransformerLM(nn.Module):
         if not self.packed and (documents is not None or prefix is not None):
             raise ValueError("TransformerLM: documents and prefix belong to packed=True")
         x = A.embedding(A.cast(self.embed, self.compute_dtype), ids)  # (B*T, d)
-        mask = (F.attention_mask(B, T, documents=documents, prefix=prefix, device=ids.device)
-                if self.packed else None)
+        mask = F.attention_mask(B, T, documents=documents, prefix=prefix) if self.packed else None
         for blk in self.blocks:
             x = A.add(x, self._attention(self._ln(x, blk["ln1"]), blk, B, T, mask))
             h = self._lin(blk["w1"], self._ln(x, blk["ln2"]), gelu=True)  # Linear + bias + GELU

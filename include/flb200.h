@@ -597,11 +597,12 @@ int flb200_attention_packed_backward(const void* qkv, const void* out, const voi
 /* Attention (Functions.cpp:1828-1891) where each query sees an interval of the keys.  Query i of q_len stands at
  * position i + k_len - q_len (q_len <= k_len: the last positions, down to a single one).
  *
- * The mask is made once per batch, on the device, and serves every layer and both directions.  documents (int32
- * [batch][k_len], or NULL): a position sees those of its own run of equal ids; ids below zero are padding, which
- * sees nothing and, by that rule, is seen by nobody else's run.  causal: position p sees p and what is before
- * it.  prefix (int32 [batch], or NULL; with causal): the row's first prefix positions are seen by all (of their
- * document).  A query that sees nothing has zeros for its output and minus infinity for its lse. */
+ * Without documents a call's descriptor says all: causal (position p sees p and what is before it) and prefix (int32
+ * [batch] on the device, or NULL; with causal: the row's first prefix positions are seen by all).  Rows packed with
+ * documents need a table, made once per batch on the device for every layer and both directions: documents is
+ * int32 [batch][k_len]; a position sees those of its own run of equal ids (causal and prefix within it); ids below
+ * zero are padding, which sees nothing and, by that rule, is seen by nobody else's run.  A query that sees nothing
+ * has zeros for its output and minus infinity for its lse. */
 size_t flb200_attention_mask_bytes(int64_t batch, int64_t q_len, int64_t k_len);
 int flb200_attention_mask(int64_t batch, int64_t q_len, int64_t k_len, int causal, const int32_t* documents,
                           const int32_t* prefix, void* mask, void* stream);
@@ -623,6 +624,8 @@ typedef struct flb200_attention_desc {
   int64_t batch, q_len, k_len, heads, kv_heads, head_dim;
   float scale, softcap;
   int32_t dtype;
+  int32_t causal;         /* these two where the call's mask is NULL */
+  const int32_t* prefix;
 } flb200_attention_desc;
 typedef struct flb200_head_tensor {
   void* data;

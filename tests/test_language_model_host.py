@@ -52,13 +52,14 @@ def test_attention_refuses_before_it_launches():
     assert L.lib.flb200_attention_mask_bytes(0, 4, 4) == 0
     assert L.lib.flb200_attention_mask_bytes(2, 300, 400) == 2 * 3 * 16 + 2 * 4 * 8 + 2 * 300 * 8
     for extents in ((0, 4, 4), (1, 0, 4), (1, 5, 4), (1, 4, 1 << 24)):
-        assert L.lib.flb200_attention_mask(*extents, 1, None, None, 16, None) == L.INVALID_ARG
-    assert L.lib.flb200_attention_mask(1, 4, 4, 1, None, None, None, None) == L.INVALID_ARG
-    assert L.lib.flb200_attention_mask(1, 4, 4, 0, None, 16, 16, None) == L.INVALID_ARG  # a prefix without causal
+        assert L.lib.flb200_attention_mask(*extents, 1, 16, None, 16, None) == L.INVALID_ARG
+    assert L.lib.flb200_attention_mask(1, 4, 4, 1, 16, None, None, None) == L.INVALID_ARG
+    assert L.lib.flb200_attention_mask(1, 4, 4, 1, None, None, 16, None) == L.INVALID_ARG  # a table is for documents
+    assert L.lib.flb200_attention_mask(1, 4, 4, 0, 16, 16, 16, None) == L.INVALID_ARG  # a prefix without causal
     ok = dict(batch=1, q_len=4, k_len=4, heads=4, kv_heads=2, head_dim=64, scale=1.0, softcap=0.0, dtype=L.BF16)
     t = L.HeadTensor(16, 1024, 256, 64)
     for more in (dict(kv_heads=3), dict(q_len=5), dict(heads=0), dict(scale=0.0), dict(scale=float("nan")),
-                 dict(softcap=-1.0)):
+                 dict(softcap=-1.0), dict(softcap=1e-35), dict(prefix=16)):
         d = L.AttentionDesc(**{**ok, **more})
         args = [C.byref(d)] + [C.byref(t)] * 3
         assert L.lib.flb200_masked_attention_forward(*args, None, 16, C.byref(t), None, None, None) == L.INVALID_ARG
