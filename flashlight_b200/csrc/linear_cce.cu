@@ -383,27 +383,36 @@ __device__ __forceinline__ void write_loss(const LossSums& s, int reduction, flo
   else if (reduction == FLB200_REDUCE_SUM) loss[0] = (float)s.loss;
 }
 
-// Joins the tiles' (maximum, sum) of 32 rows per CTA: 32 threads to a row take every 32nd part and meet in shared
-// memory (with eight to a row 13 us for 4096 rows of 250 parts, so 7).  Then the rows' losses, and what they add up to:
+// Joins the tiles' (maximum, sum) of 32 rows per CTA: a warp has all of them, or where a call has few, `few` rows (a power
+// of two) of 32 / few parts at once; the 32 warps' shares meet in shared memory (with eight warps 13 us for 4096 rows of
+// 250 parts, so 7; four rows of 784 parts 10.5 with a lane per row).  Then the rows' losses, and what they add up to:
 // of all rows where there is one CTA, else finish_loss_kernel adds the CTAs'.
 constexpr int kJoin = 32;
 __global__ void __launch_bounds__(32 * kJoin)
 join_lse_kernel(const float2* __restrict__ partial, int parts, const float* __restrict__ target_score,
                 const int32_t* __restrict__ targets, int ignore, long long classes, int rows, int reduction,
                 float* __restrict__ lse, float* __restrict__ loss, int32_t* __restrict__ count,
-                int32_t* __restrict__ bad, LossSums* __restrict__ sums) {
+                int32_t* __restrict__ bad, LossSums* __restrict__ sums, int few) {
   chain_begin();
   __shared__ float2 met[kJoin][32];
-  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, r = blockIdx.x * 32 + lane;
+  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int r = few < 32 && lane >= few ? rows : blockIdx.x * 32 + lane;  // this lane's row in what follows the parts
   float top = -FLT_MAX, sum = 0.f;
-  if (r < rows) {
+  const int at = blockIdx.x * 32 + (lane & (few - 1)), at_once = 32 / few;
+  if (at < rows) {
 #pragma unroll 4
-    for (int p = g; p < parts; p += kJoin) {
-      const float2 x = partial[(long long)p * rows + r];
+    for (int p = g * at_once + lane / few; p < parts; p += kJoin * at_once) {
+      const float2 x = partial[(long long)p * rows + at];
       const float mx = fmaxf(top, x.x);
       sum = sum * exp_below(top - mx) + x.y * exp_below(x.x - mx);
       top = mx;
     }
+  }
+  for (int o = few; o < 32; o <<= 1) {
+    const float other = __shfl_xor_sync(0xffffffffu, top, o), more = __shfl_xor_sync(0xffffffffu, sum, o);
+    const float mx = fmaxf(top, other);
+    sum = sum * exp_below(top - mx) + more * exp_below(other - mx);
+    top = mx;
   }
   met[g][lane] = make_float2(top, sum);
   for (int half = kJoin / 2; half > 0; half >>= 1) {
@@ -710,9 +719,11 @@ int flb200_linear_cce_forward(const flb200_linear_cce_desc* d, const void* x, co
     parts += (int)(tiles * groups) - (short_last ? 1 : 0);
   }
   const int blocks = (int)((s.rows + 31) / 32);
+  int few = 1;
+  while (few < 32 && few < s.rows) few *= 2;
   launch_chained(join_lse_kernel, blocks, 32 * kJoin, 0, st, scratch.partial, parts, scratch.target_score, targets,
                  d->ignore_index, s.classes, (int)s.rows, d->reduction, lse, loss, count_out, bad_target_flag,
-                 scratch.sums);
+                 scratch.sums, few);
   FLB200_AFTER_LAUNCH("linear_cce_join");
   if (blocks == 1) return FLB200_OK;
   launch_chained(finish_loss_kernel, 1, 32, 0, st, scratch.sums, blocks, d->reduction, loss, count_out,
