@@ -1066,6 +1066,7 @@ flb200_linear_cce_desc linear_cce_desc(const Tensor& in, const Tensor& w, const 
                                        int reduction, int ignore) {
   const LinearDims l = linear_dims(w, in);
   if (targets.numel() != l.cols) value_error("dimension mismatch in categorical cross entropy");
+  if (l.cols < 1 || l.I < 1 || l.O < 1) value_error("linear_cross_entropy: empty tensors");
   if (targets.scalar_type() != ScalarType::Int) value_error("linear_cross_entropy: targets are int32");
   if (w.dim() != 2 || w.scalar_type() != in.scalar_type())
     value_error("linear_cross_entropy: input and weight must be of one type");
@@ -1082,7 +1083,7 @@ NATIVE(linear_cce_forward) {
   const Tensor &in = x.tensor(0), &w = x.tensor(1), &tg = x.tensor(3);
   const Tensor* bias = x.t(2);
   const flb200_linear_cce_desc d = linear_cce_desc(in, w, bias, tg, x.n32(4), x.n32(5));
-  if (d.rows < 1 || !in.is_contiguous() || !w.is_contiguous() || !flb200_linear_cce_supported(&d)) Py_RETURN_NONE;
+  if (!in.is_contiguous() || !w.is_contiguous() || !flb200_linear_cce_supported(&d)) Py_RETURN_NONE;
   Tensor loss = floats(d.reduction == FLB200_REDUCE_NONE ? d.rows : 1, in), lse = floats(d.rows, in);
   Tensor meta = empty({2}, ScalarType::Int, in);  // [count, bad-target flag]
   int32_t* m = static_cast<int32_t*>(meta.data_ptr());

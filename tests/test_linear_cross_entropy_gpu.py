@@ -182,6 +182,7 @@ def test_refusals_and_the_chain():
                 lambda: F.linear_cross_entropy(x, w.half(), None, t),
                 lambda: F.linear_cross_entropy(x, w, torch.ones(7, device="cuda"), t),
                 lambda: F.linear_cross_entropy(x, w, torch.ones(2048, device="cuda").half(), t),
+                lambda: F.linear_cross_entropy(x[:0], w, None, t[:0]),
                 lambda: F.linear_cross_entropy(x, w, None, t, 7)):
         with pytest.raises(ValueError):
             bad()
