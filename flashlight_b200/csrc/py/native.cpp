@@ -1156,31 +1156,42 @@ NATIVE(adamw_step) {
   d.epsilon = x.d(10); d.weight_decay = x.d(11); d.grad_scale = x.d(12);
   d.state_bits = eight ? 8 : 32;
   const ScalarType state = eight ? ScalarType::Float8_e4m3fn : ScalarType::Float;
+  // (a step has hundreds of tensors, four to six for each parameter: their checks are most of a short step)
+  const at::Device here(at::kCUDA, (c10::DeviceIndex)c10::cuda::current_device());
+  const auto state_type = c10::scalarTypeToTypeMeta(state), floats_type = c10::scalarTypeToTypeMeta(ScalarType::Float);
+  const auto data = [&](c10::TensorImpl* t) {
+    if (t->device() != here)
+      value_error(t->is_cuda() ? "adamw_step: tensors must be on the current device"
+                               : "the B200 autograd extension needs device (CUDA) tensors");
+    return t->mutable_data();
+  };
   std::vector<flb200_adamw_tensor> group[3][3];
-  const int device = (int)c10::cuda::current_device();
   for (Py_ssize_t i = 0; i < params.n; ++i) {
     const Tensor& p = params.tensor(i);
     const Tensor* g = grads.t(i);
     if (!g) continue;
-    const Tensor &m = firsts.tensor(i), &v = seconds.tensor(i);
-    const int64_t n = p.numel();
-    if (!same_layout(p, *g)) value_error("adamw_step: a gradient must have its parameter's shape and layout");
-    if (m.numel() != n || v.numel() != n || m.scalar_type() != state || v.scalar_type() != state)
-      value_error("adamw_step: moments are float32, or float8_e4m3fn with scales, and as long as the parameter");
+    c10::TensorImpl *pi = p.unsafeGetTensorImpl(), *gi = g->unsafeGetTensorImpl();
+    c10::TensorImpl *mi = firsts.tensor(i).unsafeGetTensorImpl(), *vi = seconds.tensor(i).unsafeGetTensorImpl();
+    const int64_t n = pi->numel();
+    if (!(pi->is_contiguous() && gi->is_contiguous() ? pi->sizes() == gi->sizes() : same_layout(p, *g) && dense(p)))
+      value_error("adamw_step: a gradient must have its parameter's shape and layout");
+    if (mi->numel() != n || vi->numel() != n || mi->dtype() != state_type || vi->dtype() != state_type ||
+        !mi->is_contiguous() || !vi->is_contiguous())
+      value_error("adamw_step: moments are float32, or float8_e4m3fn with scales, dense and as long as the parameter");
     flb200_adamw_tensor t = {};
-    t.param = P(p); t.grad = P(*g); t.first = P(m); t.second = P(v); t.n = n;
+    t.param = data(pi); t.grad = data(gi); t.first = data(mi); t.second = data(vi); t.n = n;
     if (eight) {
-      const Tensor &a = s1.tensor(i), &b = s2.tensor(i);
+      c10::TensorImpl *ai = s1.tensor(i).unsafeGetTensorImpl(), *bi = s2.tensor(i).unsafeGetTensorImpl();
       const int64_t blocks = (n + FLB200_ADAMW_BLOCK - 1) / FLB200_ADAMW_BLOCK;
-      if (a.numel() != blocks || b.numel() != blocks || a.scalar_type() != ScalarType::Float ||
-          b.scalar_type() != ScalarType::Float)
-        value_error("adamw_step: scales are float32, one per 256 elements");
-      t.first_scale = Pf(&a); t.second_scale = Pf(&b);
+      if (ai->numel() != blocks || bi->numel() != blocks || ai->dtype() != floats_type || bi->dtype() != floats_type ||
+          !ai->is_contiguous() || !bi->is_contiguous())
+        value_error("adamw_step: scales are float32, dense, one per 256 elements");
+      t.first_scale = static_cast<float*>(data(ai));
+      t.second_scale = static_cast<float*>(data(bi));
     }
-    if (p.get_device() != device || g->get_device() != device || m.get_device() != device ||
-        v.get_device() != device)
-      value_error("adamw_step: tensors must be on the current device");
-    group[code_of(p)][code_of(*g)].push_back(t);
+    auto& to = group[code_of(p)][code_of(*g)];
+    if (to.empty()) to.reserve((size_t)(params.n - i));
+    to.push_back(t);
   }
   for (int pt = 0; pt < 3; ++pt)
     for (int gt = 0; gt < 3; ++gt) {
