@@ -167,7 +167,8 @@ SIGNATURES = {
     "flb200_attention_mask": (C.c_int, [i64, i64, i64, C.c_int, vp, vp, vp, vp]),
     "flb200_masked_attention_supported": (C.c_int, [P(AttentionDesc)]),
     "flb200_masked_attention_forward": (C.c_int, [P(AttentionDesc), P(HeadTensor), P(HeadTensor), P(HeadTensor),
-                                                  vp, vp, P(HeadTensor), vp, vp, vp]),
+                                                  vp, vp, P(HeadTensor), vp, vp, vp, sz, vp]),
+    "flb200_masked_attention_forward_workspace_bytes": (sz, [P(AttentionDesc)]),
     "flb200_masked_attention_backward_workspace_bytes": (sz, [P(AttentionDesc)]),
     "flb200_masked_attention_backward": (C.c_int, [P(AttentionDesc)] + [P(HeadTensor)] * 4 +
                                          [vp, P(HeadTensor), vp, vp, vp] +

@@ -425,6 +425,12 @@ struct AttnFwdArgs {
   OutTensor out;
   void* rest;  // [batch][q_len][heads][head_dim]: what out's rounding took, or null
   float* lse;  // [batch][heads][q_len], or null
+  // Few queries behind many keys: `splits` CTAs share a query block's keys, each leaves its rows' output and lse (in
+  // powers of 2) in fp32, [split][batch][heads][q_len][D] and [split][batch][heads][q_len], and join_splits_kernel joins
+  // them.
+  int splits, ctas;  // ctas: of one split
+  float* part;
+  float* part_lse;
 };
 
 template <int D, typename T, bool CAP, bool BIAS>
@@ -450,12 +456,17 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int nq = blocks_of(a.s.q_len), off = a.s.k_len - a.s.q_len;
-  const int all_heads = gridDim.x / nq;
-  const int i = nq - 1 - (int)blockIdx.x / all_heads;  // of all heads the longest of a causal mask first
-  const int bh = blockIdx.x % all_heads, batch = bh / a.s.heads, head = bh - batch * a.s.heads;
+  const int all_heads = a.ctas / nq, split = blockIdx.x / a.ctas, cta = blockIdx.x - split * a.ctas;
+  const int i = nq - 1 - cta / all_heads;  // of all heads the longest of a causal mask first
+  const int bh = cta % all_heads, batch = bh / a.s.heads, head = bh - batch * a.s.heads;
   const int4 info = a.s.mask.q_block(batch, i);
-  const int begin = info.y > info.x ? info.x / kBlock : 0;
-  const int blocks = info.y > info.x ? blocks_of(info.y) - begin : 0;
+  int begin = info.y > info.x ? info.x / kBlock : 0;
+  int blocks = info.y > info.x ? blocks_of(info.y) - begin : 0;
+  if (a.splits > 1) {
+    const int each = (blocks + a.splits - 1) / a.splits;
+    begin += split * each;
+    blocks = max(0, min(each, blocks - split * each));
+  }
 
   const int kv = head / a.s.group;
   auto load = [&](int j, uint32_t s, bool k, bool v) {
@@ -687,6 +698,7 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     lost = half == 0 ? lost + met[128] : met[0] + lost;
     if (blocks > 0) wait(bar_o, (blocks - 1) & 1, 10);
     const float inv = sum > 0.f ? 1.f / (sum - lost) : sum;  // (a sum that is not a number shows in the output)
+    const long long part_row = ((long long)split * all_heads + bh) * a.s.q_len + q;
     const long long rest_at = (((long long)batch * a.s.q_len + q) * a.s.heads + head) * a.s.head_dim;
 #pragma unroll 1
     for (int c = 0; c < D / 2; c += 16) {
@@ -700,12 +712,23 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[e] = 0;
       }
-      if (q < a.s.q_len)
+      if (q >= a.s.q_len) continue;
+      if (a.splits > 1) {
+        float4* to = reinterpret_cast<float4*>(a.part + (part_row * D + D / 2 * half + c));
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          to[e / 4] = make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
+                                  __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+      } else {
         store16_of<T>(a.out, batch, q, head, D / 2 * half + c, a.s.head_dim, o, inv,
                       a.rest ? static_cast<T*>(a.rest) + rest_at : nullptr);
+      }
     }
-    if (half == 0 && q < a.s.q_len && a.lse)
-      a.lse[(long long)bh * a.s.q_len + q] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * kLn2;
+    if (half == 0 && q < a.s.q_len) {
+      const float lse = sum == 0.f ? -INFINITY : ref + log2f(sum);
+      if (a.splits > 1) a.part_lse[part_row] = lse;
+      else if (a.lse) a.lse[(long long)bh * a.s.q_len + q] = lse * kLn2;
+    }
   }
   if (*failed)  // copies and contractions under way when a wait ran out have ended after this
     for (const long long t0 = clock64(); clock64() - t0 < 100000;) {
@@ -717,6 +740,43 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     tc_fence_after();
     tmem_dealloc(tmem, 256);
   }
+}
+
+// A warp joins a row's splits: o = sum_s w_s o_s / sum_s w_s with w_s = 2^(lse_s - max lse).  Four columns a lane at 128.
+template <int D, typename T>
+__global__ void __launch_bounds__(256)
+join_splits_kernel(const AttnFwdArgs a, long long rows) {
+  chain_begin();
+  constexpr int kPer = D / 32;
+  const long long r = (blockIdx.x * 256LL + threadIdx.x) >> 5;  // [batch][heads][q_len]
+  const int lane = threadIdx.x & 31;
+  if (r >= rows) return;
+  float top = -1e30f;
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_lse[s * rows + r]);
+  float o[kPer], sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) o[e] = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float w = ex2(a.part_lse[s * rows + r] - top);
+    sum += w;
+    const float* from = a.part + (s * rows + r) * D + kPer * lane;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) o[e] = fmaf(w, from[e], o[e]);
+  }
+  const long long bh = r / a.s.q_len, b = bh / a.s.heads;
+  const int q = (int)(r - bh * a.s.q_len), h = (int)(bh - b * a.s.heads), c0 = kPer * lane;
+  const float inv = sum > 0.f ? 1.f / sum : sum;
+  T* to = static_cast<T*>(a.out.p) + b * a.out.batch + q * a.out.row + h * a.out.head;
+  T* rest = a.rest ? static_cast<T*>(a.rest) + ((b * a.s.q_len + q) * a.s.heads + h) * a.s.head_dim : nullptr;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    if (c0 + e >= a.s.head_dim) continue;
+    const float x = o[e] * inv;
+    const T t = Num<T>::from_f(x);
+    to[c0 + e] = t;
+    if (rest) rest[c0 + e] = Num<T>::from_f(x - Num<T>::to_f(t));
+  }
+  if (lane == 0 && a.lse) a.lse[r] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 // ------------------------------------------------------------------------------------------ gradient
@@ -1120,6 +1180,15 @@ OutTensor out_of(const flb200_head_tensor& t, long long head_dim) {
   return OutTensor{t.data, t.batch, t.row, t.head, wide ? 1 : 0};
 }
 
+// Of how many parts each query block's keys are: as many as fill the SMs' two places each, of four blocks at least.  (Less
+// than that the second launch costs more than it saves.)
+int splits_of(const flb200_attention_desc* d) {
+  const long long ctas = d->batch * d->heads * blocks_of(d->q_len), places = 2LL * device_info().sm_count;
+  const long long s = std::min(places / ctas, (long long)blocks_of(d->k_len) / 4);
+  return s < 2 ? 1 : (int)s;
+}
+int padded_dim(const flb200_attention_desc* d) { return d->head_dim <= 64 ? 64 : 128; }
+
 AttnShape shape_of(const flb200_attention_desc* d, const float* slopes, const void* mask) {
   AttnShape s{};
   s.q_len = (int)d->q_len;
@@ -1166,9 +1235,15 @@ int launch_forward(const flb200_attention_desc* d, const CUtensorMap& mq, const 
                    AttnFwdArgs a, cudaStream_t st) {
   const auto kernel = masked_forward_kernel<D, T, CAP, BIAS>;
   if (int rc = configure(reinterpret_cast<const void*>(kernel), FwdSmem<D>::kTotal)) return rc;
-  launch_chained(kernel, (unsigned)(d->batch * d->heads * blocks_of(d->q_len)), kFwdThreads, FwdSmem<D>::kTotal, st, mq, mk, mv, a);
+  a.ctas = (int)(d->batch * d->heads * blocks_of(d->q_len));
+  launch_chained(kernel, (unsigned)(a.ctas * a.splits), kFwdThreads, FwdSmem<D>::kTotal, st, mq, mk, mv, a);
   FLB200_AFTER_LAUNCH("masked_attention_forward");
   count_tc_launch();
+  if (a.splits > 1) {
+    const long long rows = d->batch * d->heads * d->q_len;
+    launch_chained(join_splits_kernel<D, T>, (unsigned)((rows + 7) / 8), 256, 0, st, a, rows);
+    FLB200_AFTER_LAUNCH("masked_attention_join");
+  }
   return FLB200_OK;
 }
 template <int D, int UNITS, typename T, bool CAP, bool BIAS>
@@ -1247,10 +1322,16 @@ int flb200_masked_attention_supported(const flb200_attention_desc* d) {
              : 0;
 }
 
+size_t flb200_masked_attention_forward_workspace_bytes(const flb200_attention_desc* d) {
+  if (!d || d->batch < 1 || d->heads < 1 || d->q_len < 1 || d->k_len < 1) return 0;
+  const long long splits = splits_of(d);
+  return splits < 2 ? 0 : (size_t)(splits * d->batch * d->heads * d->q_len * (padded_dim(d) + 1)) * sizeof(float);
+}
+
 int flb200_masked_attention_forward(const flb200_attention_desc* d, const flb200_head_tensor* q,
                                     const flb200_head_tensor* k, const flb200_head_tensor* v, const float* slopes,
                                     const void* mask, const flb200_head_tensor* out, void* rest, float* lse,
-                                    void* stream) {
+                                    void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_attention("masked_attention_forward", d)) return rc;
   FLB200_REQUIRE(!mask || aligned16(mask), "masked_attention_forward: the mask must be 16-byte aligned");
   FLB200_REQUIRE(!rest || aligned16(rest), "masked_attention_forward: rest must be 16-byte aligned");
@@ -1266,6 +1347,14 @@ int flb200_masked_attention_forward(const flb200_attention_desc* d, const flb200
   a.out = out_of(*out, d->head_dim);
   a.rest = rest;
   if (reinterpret_cast<uintptr_t>(rest) & 31) a.out.wide = 0;
+  a.splits = splits_of(d);
+  const size_t need = flb200_masked_attention_forward_workspace_bytes(d);
+  if (need) {
+    if (!workspace || !aligned16(workspace) || workspace_bytes < need)
+      return fail(FLB200_WORKSPACE_TOO_SMALL, "masked_attention_forward: workspace %zu < %zu", workspace_bytes, need);
+    a.part = static_cast<float*>(workspace);
+    a.part_lse = a.part + a.splits * d->batch * d->heads * d->q_len * padded_dim(d);
+  }
   a.lse = lse;
   return dispatch(d, slopes != nullptr, [&](auto dim, auto type, auto cap, auto bias) {
     return launch_forward<decltype(dim)::value, decltype(type), decltype(cap)::value, decltype(bias)::value>(

@@ -720,9 +720,10 @@ NATIVE(masked_attention) {  // (AttentionCall's, train) -> (out, lse, rest), the
     rest = empty_like(out);
   }
   const Heads o(out, "out");
+  Workspace ws(flb200_masked_attention_forward_workspace_bytes(&d), q);
   check(unlocked(flb200_masked_attention_forward, &d, (const flb200_head_tensor*)&c.q.h,
                  (const flb200_head_tensor*)&c.k.h, (const flb200_head_tensor*)&c.v.h, c.slopes, c.mask, &o.h,
-                 rest.defined() ? P(rest) : nullptr, lse.defined() ? Pf(&lse) : nullptr, stream()));
+                 rest.defined() ? P(rest) : nullptr, lse.defined() ? Pf(&lse) : nullptr, ws.p(), ws.bytes, stream()));
   return wrap({out, lse, rest});
 }
 // (AttentionCall's, out, rest, grad_out, lse, grad_q, grad_k, grad_v or None three times: new tensors)

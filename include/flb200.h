@@ -632,10 +632,13 @@ typedef struct flb200_head_tensor {
   int64_t batch, row, head; /* strides */
 } flb200_head_tensor;
 int flb200_masked_attention_supported(const flb200_attention_desc* d);
+/* (0 unless there are few queries and many keys, whose blocks are then shared out and joined) */
+size_t flb200_masked_attention_forward_workspace_bytes(const flb200_attention_desc* d);
 int flb200_masked_attention_forward(const flb200_attention_desc* d, const flb200_head_tensor* q,
                                     const flb200_head_tensor* k, const flb200_head_tensor* v,
                                     const float* slopes, const void* mask, const flb200_head_tensor* out,
-                                    void* rest, float* lse, void* stream);
+                                    void* rest, float* lse, void* workspace, size_t workspace_bytes,
+                                    void* stream);
 size_t flb200_masked_attention_backward_workspace_bytes(const flb200_attention_desc* d);
 int flb200_masked_attention_backward(const flb200_attention_desc* d, const flb200_head_tensor* q,
                                      const flb200_head_tensor* k, const flb200_head_tensor* v,

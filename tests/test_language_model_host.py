@@ -62,12 +62,13 @@ def test_attention_refuses_before_it_launches():
                  dict(softcap=-1.0), dict(softcap=1e-35), dict(prefix=16)):
         d = L.AttentionDesc(**{**ok, **more})
         args = [C.byref(d)] + [C.byref(t)] * 3
-        assert L.lib.flb200_masked_attention_forward(*args, None, 16, C.byref(t), None, None, None) == L.INVALID_ARG
+        assert L.lib.flb200_masked_attention_forward(*args, None, 16, C.byref(t), None, None, None, 0,
+                                                     None) == L.INVALID_ARG
     for more in (dict(head_dim=65), dict(head_dim=136), dict(dtype=L.F32)):
         d = L.AttentionDesc(**{**ok, **more})
         assert L.lib.flb200_masked_attention_supported(C.byref(d)) == 0
         assert L.lib.flb200_masked_attention_forward(C.byref(d), C.byref(t), C.byref(t), C.byref(t), None, 16, C.byref(t),
-                                                     None, None, None) == L.UNSUPPORTED
+                                                     None, None, None, 0, None) == L.UNSUPPORTED
 
 
 def test_packed_batches():

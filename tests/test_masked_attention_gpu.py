@@ -91,6 +91,10 @@ CASES = [
     (1, 130, 515, 2, 2, 64, True, 0, False, 0.0, True),
     (1, 33, 513, 2, 2, 40, False, 200, False, 0.0, False),
     (1, 1100, 1100, 1, 1, 64, True, 0, False, 0.0, False),
+    (1, 1, 5000, 4, 2, 64, True, 0, False, 0.0, False),     # keys shared out among CTAs and joined
+    (2, 3, 3000, 2, 1, 128, True, 700, False, 15.0, True),  # (some have no key of the query's document)
+    (1, 140, 2000, 1, 1, 72, False, 900, False, 0.0, False),
+    (1, 2, 1030, 1, 1, 16, True, 0, True, 0.0, False),
 ]
 
 
