@@ -245,10 +245,12 @@ __device__ __forceinline__ void exp2_by_fma(F2 z, float& a, float& b) {
   b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
 }
 // One pair of a row's exponentials in this many is made so, the others by the special function unit (0: all).  At 64
-// dimensions that unit is the busiest, at 128 the tensor pipe, but with a cap, which takes two more of it a score.  16 heads of 8192 causal positions, us: forward at 64
-// 195 with none, 190 with one in eight, 182 in four, 206 in two; with a distance bias (12 heads, documents of 3000) 106, 101,
-// 110, 122; gradient 524, 505, 519, 552; forward at 128 246, 258, 268, 276; 2 x 1500 with a cap at 128 forward 57, 49, 53,
-// 60, gradient 150, 128, 142, 144.
+// dimensions that unit is the busiest, at 128 the tensor pipe, but with a cap, which takes two more of it a score.
+// us with none, one in eight, in four, in two:
+//   16 heads of 8192 causal positions of 64, forward 195, 190, 182, 206; gradient 524, 505, 519, 552
+//   12 in documents of 3000 with a distance bias, forward 106, 101, 110, 122
+//   16 of 8192 of 128, forward 246, 258, 268, 276
+//   2 x 1500, a cap, 16 of 128, forward 57, 49, 53, 60; gradient 150, 128, 142, 144
 constexpr int forward_by_fma(int D, bool cap, bool bias) { return cap ? 8 : D == 64 ? (bias ? 8 : 4) : 0; }
 constexpr int gradient_by_fma(int D, bool cap) { return D == 64 || cap ? 8 : 0; }
 template <typename T>

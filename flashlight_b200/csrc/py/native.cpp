@@ -682,6 +682,9 @@ struct AttentionCall {
     if (tk.sizes() != tv.sizes() || tq.size(0) != tk.size(0) || tq.size(3) != tk.size(3) ||
         tq.scalar_type() != tk.scalar_type() || tq.scalar_type() != tv.scalar_type())
       value_error("masked_attention: q, k and v must be of one type, batch and head dim, k and v alike");
+    for (const Tensor* t : {&tk, &tv, s, x.t(9)})
+      if (t && t->get_device() != tq.get_device())
+        value_error("masked_attention: tensors must be on one device");
     if (tk.size(2) < 1 || tq.size(2) < 1 || tq.size(2) % tk.size(2) != 0)
       value_error("masked_attention: the query heads must be a multiple of the key heads");
     d.batch = x.i(5);
