@@ -226,13 +226,20 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// (fmaxf and max.f32 would drop a NaN)
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 // 2^z of two numbers below 2^7 on the FMA pipe: Cody and Waite's reduction to [-1/2, 1/2], a polynomial of degree 4 (the
-// one of the least relative error, 2.6e-6, from Remez' exchange), and the exponent added to its bits.  Below -126 the
-// result stays at 2^-126.
+// one of the least relative error, 2.6e-6, from Remez' exchange), and a product with the power of two that has the
+// integer for its exponent.  At -127 that power's bits are zero, so what is smaller gives zero; a NaN stays one, through
+// the clamp and the product (added to a NaN's bits the exponent would make a finite number of it).
 __device__ __forceinline__ void exp2_by_fma(F2 z, float& a, float& b) {
   float z0, z1, t0, t1;
   unpair(z, z0, z1);
-  z = pair(fmaxf(z0, -126.f), fmaxf(z1, -126.f));
+  z = pair(max_or_nan(z0, -127.f), max_or_nan(z1, -127.f));
   const F2 t = z + pair(12582912.f);  // 1.5 * 2^23: the nearest integer is in the low bits
   const F2 f = z + fused(t, pair(-1.f), pair(12582912.f));
   F2 p = fused(f, pair(0.009570102207362652f), pair(0.05591785907745361f));
@@ -240,9 +247,9 @@ __device__ __forceinline__ void exp2_by_fma(F2 z, float& a, float& b) {
   p = fused(p, f, pair(0.6931217908859253f));
   p = fused(p, f, pair(0.9999992847442627f));
   unpair(t, t0, t1);
+  p = p * pair(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u),
+               __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u));
   unpair(p, a, b);
-  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
-  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
 }
 // One pair of a row's exponentials in this many is made so, the others by the special function unit (0: all).  At 64
 // dimensions that unit is the busiest, at 128 the tensor pipe, but with a cap, which takes two more of it a score.
