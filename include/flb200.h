@@ -706,7 +706,8 @@ typedef struct flb200_linear_cce_desc {
   int32_t dtype;
 } flb200_linear_cce_desc;
 int flb200_linear_cce_supported(const flb200_linear_cce_desc* d);
-/* which: 0 forward, 1 backward; depends on the alignment of x and weight */
+/* which: 0 forward, 1 backward; depends on the alignment of x and weight.  Forward's workspace must be 16-byte
+ * aligned, backward's 32-byte aligned; else FLB200_WORKSPACE_TOO_SMALL. */
 size_t flb200_linear_cce_workspace_bytes(const flb200_linear_cce_desc* d, const void* x, const void* weight,
                                          int which);
 int flb200_linear_cce_forward(const flb200_linear_cce_desc* d, const void* x, const void* weight,
