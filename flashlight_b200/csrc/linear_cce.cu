@@ -462,7 +462,9 @@ finish_loss_kernel(const LossSums* __restrict__ sums, int n, int reduction, floa
   if (threadIdx.x == 0) write_loss(all, reduction, loss, count, bad);
 }
 
-// Each row's RowInfo, its weight step * g_r / max |g|, zero where the row does not count; factor = max |g| / step
+// Each row's RowInfo, its weight step * g_r / max |g| over the finite g, zero where the row does not count; factor =
+// max |g| / step.  A g that is not finite is its row's weight itself: the row's entries are then not finite in any type,
+// and the others' are as without it.
 __global__ void __launch_bounds__(1024)
 row_weights_kernel(const float* __restrict__ grad_loss, const int32_t* __restrict__ targets,
                    const int32_t* __restrict__ count, const float* __restrict__ lse, int reduction, int ignore,
@@ -470,23 +472,28 @@ row_weights_kernel(const float* __restrict__ grad_loss, const int32_t* __restric
                    float* __restrict__ factor) {
   chain_begin();
   __shared__ float scratch[32];
-  float top = 0.f;
+  float top = 0.f, all = 0.f;  // all: what every row has, where the loss is reduced
   if (reduction == FLB200_REDUCE_NONE) {  // (one CTA)
     for (int r = threadIdx.x; r < rows; r += 1024)
-      if (counts(targets[r], ignore, classes)) top = fmaxf(top, fabsf(grad_loss[r]));
+      if (counts(targets[r], ignore, classes) && isfinite(grad_loss[r])) top = fmaxf(top, fabsf(grad_loss[r]));
     top = warp_max(top);
     if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = top;
     __syncthreads();
     top = warp_max(scratch[threadIdx.x & 31]);
   } else {
-    top = grad_loss[0];
-    if (reduction == FLB200_REDUCE_MEAN) top = *count > 0 ? top / (float)*count : 0.f;
+    all = grad_loss[0];
+    if (reduction == FLB200_REDUCE_MEAN) all = *count > 0 ? all / (float)*count : 0.f;
+    top = isfinite(all) ? all : 1.f;
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) *factor = top / step;
   for (int r = blockIdx.x * 1024 + threadIdx.x; r < rows; r += gridDim.x * 1024) {
     float w = 0.f;
-    if (counts(targets[r], ignore, classes))
-      w = reduction != FLB200_REDUCE_NONE ? step : (top > 0.f ? step * (grad_loss[r] / top) : 0.f);
+    if (counts(targets[r], ignore, classes)) {
+      const float g = reduction != FLB200_REDUCE_NONE ? all : grad_loss[r];
+      if (!isfinite(g)) w = g;
+      else if (reduction != FLB200_REDUCE_NONE) w = step;
+      else w = top > 0.f ? step * (g / top) : 0.f;
+    }
     info[r] = RowInfo{lse[r] * kLog2e, w, targets[r], 0};
   }
 }
