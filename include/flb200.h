@@ -697,8 +697,10 @@ int flb200_scores_cce_backward(const void* x, const float* lse, const float* gra
  * the log of the sum of each row's exponentials; backward makes the scores again, a piece of the vocabulary at a
  * time.  FLB200_F16 or FLB200_BF16 tensors, any extents and alignment; scores, statistics and sums in fp32;
  * the scores' gradient is rounded to the tensors' type once, relative to the largest row weight.  Loss, count,
- * reductions and targets out of range as flb200_cce_forward (the flag is written either way); a row whose target
- * is ignored or out of range adds nothing to any gradient.  Of the gradients any may be NULL; grad_w is of the weights' type or f32. */
+ * reductions and targets out of range as flb200_cce_forward (the flag is written either way).  A row whose target is
+ * ignored or out of range adds nothing to any gradient, and its scores may be anything; but grad_w is x^T times
+ * that row's zeros, so there its x must be finite, or grad_w is not.  Of the gradients any may be NULL; grad_w is of
+ * the weights' type or f32. */
 typedef struct flb200_linear_cce_desc {
   int64_t rows, features, classes;
   int32_t reduction;     /* FLB200_REDUCE_* */
