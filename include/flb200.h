@@ -614,10 +614,14 @@ int flb200_attention_mask(int64_t batch, int64_t q_len, int64_t k_len, int causa
  * probabilities and the scores' gradient are rounded to the tensors' type as operands (in f16 the latter must
  * stay below 65504, as the gradients themselves must).  Tensors by strides in
  * elements, each a multiple of 8, data 16-byte aligned: element (b, t, h, d) at b*batch + t*row + h*head + d.
- * The values of k and v in a block of 128 positions that some query of a block sees must be finite, or that
- * query block's output is not.  For the gradient forward keeps lse, fp32 [batch][heads][q_len], and rest
- * [batch][q_len][heads][head_dim], what the rounding of out took, in the tensors' type; either may be NULL, and
- * without rest the gradient of the scores carries a rounding of out more.
+ * What the mask leaves out has weight zero whatever its score, but the products multiply values by those zeros.  So
+ * where some query of a block of 128 sees a part of a block of 128 keys, all of that block's v must be finite, or the
+ * query block's output is not; backward, its k must be too, or the query block's grad_q is not, and the query
+ * block's q and grad_out (those of padding and of rows that see nothing included), or the key block's grad_k and
+ * grad_v are not.  Pairs of blocks that have nothing to do with one another may hold anything.
+ * For the gradient forward keeps lse, fp32 [batch][heads][q_len], and rest [batch][q_len][heads][head_dim], what the
+ * rounding of out took, in the tensors' type; either may be NULL, and without rest the gradient of the scores carries
+ * a rounding of out more.
  * Backward gives the gradients of q, k and v (those of k and v summed over the heads that share them), without
  * atomics: equal inputs give equal bits. */
 typedef struct flb200_attention_desc {

@@ -54,3 +54,34 @@ def test_visible_key_of_one_query(D):
         for a, b in zip(got[:2], clean[:2]):
             a, b = a.reshape(H, -1), b.reshape(H, -1)
             assert torch.equal(a[0], b[0]) and bool(torch.isnan(a[1]).all()), at
+
+
+def test_behind_the_mask_in_the_gradient():
+    """Padding of a whole block and more: nothing of its q, k, v and of its output's gradient reaches another row.  In
+    blocks that are partly seen, a key behind the mask may have any score."""
+    from flashlight_b200 import functions as F
+    B, T, H, D = 2, 600, 2, 64
+    g = torch.Generator("cuda").manual_seed(4)
+    q, k, v, go = (torch.randn(B, T, H, D, generator=g, device="cuda").bfloat16() for _ in range(4))
+    ids = torch.zeros(B, T, dtype=torch.int32)
+    ids[:, 130:] = 1
+    ids[:, 384:] = -1
+    mask = F.attention_mask(B, T, documents=ids.cuda())
+
+    def both(q, k, v, go):
+        out, lse, rest = F.masked_attention(q, k, v, mask, 0.125)
+        return (out,) + tuple(F.masked_attention_backward(q, k, v, out, rest, go, lse, mask, 0.125))
+
+    clean = both(q, k, v, go)
+    bad = [t.clone() for t in (q, k, v, go)]
+    for t, value in zip(bad, ("nan", "nan", "inf", "inf")):
+        t[:, 384:] = float(value)
+    for name, got, want in zip(("out", "dq", "dk", "dv"), both(*bad), clean):
+        assert torch.equal(got, want), name
+        assert bool((got[:, 384:] == 0).all()) and bool(torch.isfinite(got).all()), name
+    # the first document's end is inside a block: behind it the second document's queries see nothing of the first
+    far = k.clone()
+    far[:, 128:130] = float("nan")
+    out, lse, _ = F.masked_attention(q, far, v, mask, 0.125)
+    assert torch.equal(out[:, 130:384], clean[0][:, 130:384]) and bool(torch.isnan(out[:, 129]).all())
+    assert torch.equal(out[:, :128], clean[0][:, :128])
