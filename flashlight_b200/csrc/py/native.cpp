@@ -1197,13 +1197,29 @@ NATIVE(adamw_step) {
     if (to.empty()) to.reserve((size_t)(params.n - i));
     to.push_back(t);
   }
-  for (int pt = 0; pt < 3; ++pt)
-    for (int gt = 0; gt < 3; ++gt) {
-      const auto& ts = group[pt][gt];
-      if (ts.empty()) continue;
-      d.param_dtype = pt; d.grad_dtype = gt;
-      check(unlocked(flb200_adamw_step, (const flb200_adamw_desc*)&d, ts.data(), (int64_t)ts.size(), stream()));
-    }
+  // A call that is refused has changed nothing: the types, the numbers and the alignment of all groups are looked at
+  // before the first group is launched (the rest of what the library checks is so by what was checked above).
+  const auto bytes = [](int type) { return type == FLB200_F32 ? 4u : 2u; };
+  int groups = 0;
+  for (const auto& row : group)
+    for (const auto& ts : row) groups += !ts.empty();
+  for (const bool launch : {false, true})
+    for (int pt = 0; pt < 3; ++pt)
+      for (int gt = 0; gt < 3; ++gt) {
+        const auto& ts = group[pt][gt];
+        if (ts.empty() || (!launch && groups == 1)) continue;
+        d.param_dtype = pt; d.grad_dtype = gt;
+        if (launch) {
+          check(unlocked(flb200_adamw_step, (const flb200_adamw_desc*)&d, ts.data(), (int64_t)ts.size(), stream()));
+          continue;
+        }
+        check(flb200_adamw_step(&d, nullptr, 0, nullptr));
+        for (const flb200_adamw_tensor& t : ts)
+          if (reinterpret_cast<uintptr_t>(t.param) % bytes(pt) || reinterpret_cast<uintptr_t>(t.grad) % bytes(gt) ||
+              (!eight && (reinterpret_cast<uintptr_t>(t.first) | reinterpret_cast<uintptr_t>(t.second)) % 4) ||
+              (reinterpret_cast<uintptr_t>(t.first_scale) | reinterpret_cast<uintptr_t>(t.second_scale)) % 4)
+            value_error("adamw_step: tensors must be aligned to their elements");
+      }
   Py_RETURN_NONE;
 }
 

@@ -80,13 +80,13 @@ class AdamWOptimizer:
         return buffer, [part[:t.numel()] for part, t in zip(parts, tensors)]
 
     def step(self, grad_scale: float = 1.0) -> None:
-        self.steps += 1
         grads = [p.grad for p in self.parameters]
         F.adamw_step([p.tensor for p in self.parameters],
                      [g if g is None or g.is_contiguous() else g.contiguous() for g in grads], self.firsts,
-                     self.seconds, step=self.steps, lr=self.lr, beta1=self.beta1, beta2=self.beta2, eps=self.eps,
+                     self.seconds, step=self.steps + 1, lr=self.lr, beta1=self.beta1, beta2=self.beta2, eps=self.eps,
                      weight_decay=self.wd, grad_scale=grad_scale, first_scales=self.first_scales,
                      second_scales=self.second_scales)
+        self.steps += 1  # (a step that was refused has changed nothing and does not count)
 
     def zeroGrad(self) -> None:
         for p in self.parameters:
