@@ -161,6 +161,14 @@ void* P(const Tensor* t) {
 }
 void* P(const Tensor& t) { return P(&t); }
 float* Pf(const Tensor* t) { return static_cast<float*>(P(t)); }
+// The tensors of a call (null ones are passed over) are on the first one's device; before anything of them is looked at.
+void one_device(const char* call, const Tensor& first, std::initializer_list<const Tensor*> others) {
+  for (const Tensor* t : others)
+    if (t && t->get_device() != first.get_device()) {
+      PyErr_Format(PyExc_ValueError, "%s: tensors must be on one device", call);
+      throw PyRaised();
+    }
+}
 bool aligned16(const Tensor* t) {
   return !t || (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0;
 }
@@ -636,6 +644,7 @@ const int32_t* ints(const Tensor* t, int64_t n, const char* what) {
 NATIVE(attention_mask) {
   const int64_t B = x.i(0), q = x.i(1), k = x.i(2);
   if (B < 1 || q < 1 || k < q) value_error("attention_mask: batch >= 1 and 1 <= q_len <= k_len");
+  if (x.t(4)) one_device("attention_mask", x.tensor(4), {x.t(5)});
   const int32_t *docs = ints(x.t(4), B * k, "documents"), *prefix = ints(x.t(5), B, "prefix");
   if (prefix && !x.b(3)) value_error("attention_mask: a prefix belongs to a causal mask");
   if (!docs) Py_RETURN_NONE;
@@ -675,16 +684,18 @@ struct AttentionCall {
   flb200_attention_desc d = {};
   const float* slopes = nullptr;
   const void* mask = nullptr;
+  static const Tensor& same_device(const Args& x) {  // q
+    one_device("masked_attention", x.tensor(0), {&x.tensor(1), &x.tensor(2), x.t(3), x.t(4), x.t(9)});
+    return x.tensor(0);
+  }
   // args: q, k, v, slopes or None, mask or None, its (batch, q_len, k_len, causal, prefix or None), scale, softcap
-  explicit AttentionCall(const Args& x) : q(x.tensor(0), "q"), k(x.tensor(1), "k"), v(x.tensor(2), "v") {
+  explicit AttentionCall(const Args& x)
+      : q(same_device(x), "q"), k(x.tensor(1), "k"), v(x.tensor(2), "v") {
     const Tensor &tq = x.tensor(0), &tk = x.tensor(1), &tv = x.tensor(2);
     const Tensor *s = x.t(3), *m = x.t(4);
     if (tk.sizes() != tv.sizes() || tq.size(0) != tk.size(0) || tq.size(3) != tk.size(3) ||
         tq.scalar_type() != tk.scalar_type() || tq.scalar_type() != tv.scalar_type())
       value_error("masked_attention: q, k and v must be of one type, batch and head dim, k and v alike");
-    for (const Tensor* t : {&tk, &tv, s, x.t(9)})
-      if (t && t->get_device() != tq.get_device())
-        value_error("masked_attention: tensors must be on one device");
     if (tk.size(2) < 1 || tq.size(2) < 1 || tq.size(2) % tk.size(2) != 0)
       value_error("masked_attention: the query heads must be a multiple of the key heads");
     d.batch = x.i(5);
@@ -701,9 +712,8 @@ struct AttentionCall {
     d.softcap = (float)x.d(11);
     d.dtype = code_of(tq);
     if (m) {
-      if (m->get_device() != tq.get_device() ||
-          m->numel() != (int64_t)flb200_attention_mask_bytes(d.batch, d.q_len, d.k_len))
-        value_error("masked_attention: the mask is on another device or of other extents");
+      if (m->numel() != (int64_t)flb200_attention_mask_bytes(d.batch, d.q_len, d.k_len))
+        value_error("masked_attention: the mask is of other extents");
       mask = m->data_ptr();
     }
     if (s) {
@@ -732,14 +742,15 @@ NATIVE(masked_attention) {  // (AttentionCall's, train) -> (out, lse, rest), the
 // (AttentionCall's, out, rest, grad_out, lse, grad_q, grad_k, grad_v or None three times: new tensors)
 //   -> (grad_q, grad_k, grad_v)
 NATIVE(masked_attention_backward) {
-  AttentionCall c(x);
-  const flb200_attention_desc& d = c.d;
   const Tensor &out = x.tensor(12), &gy = x.tensor(14), &lse = x.tensor(15);
   const Tensor* rest = x.t(13);
+  one_device("masked_attention", x.tensor(0), {&out, rest, &gy, &lse, x.t(16), x.t(17), x.t(18)});
+  AttentionCall c(x);
+  const flb200_attention_desc& d = c.d;
   if (out.sizes() != x.tensor(0).sizes() || gy.sizes() != out.sizes() || gy.scalar_type() != out.scalar_type() ||
       out.scalar_type() != x.tensor(0).scalar_type())
     value_error("masked_attention: the output's gradient must be like the output");
-  if (lse.numel() != d.batch * d.heads * d.q_len || lse.scalar_type() != ScalarType::Float)
+  if (lse.numel() != d.batch * d.heads * d.q_len || lse.scalar_type() != ScalarType::Float || !lse.is_contiguous())
     value_error("masked_attention: lse does not belong to these tensors");
   if (rest && (rest->numel() != out.numel() || rest->scalar_type() != out.scalar_type() || !rest->is_contiguous()))
     value_error("masked_attention: rest does not belong to these tensors");
@@ -1068,6 +1079,7 @@ NATIVE(batchnorm_add_relu_backward) {
 // linear + logSoftmax + cross entropy without the scores
 flb200_linear_cce_desc linear_cce_desc(const Tensor& in, const Tensor& w, const Tensor* bias, const Tensor& targets,
                                        int reduction, int ignore) {
+  one_device("linear_cross_entropy", in, {&w, bias, &targets});
   const LinearDims l = linear_dims(w, in);
   if (targets.numel() != l.cols) value_error("dimension mismatch in categorical cross entropy");
   if (l.cols < 1 || l.I < 1 || l.O < 1) value_error("linear_cross_entropy: empty tensors");
@@ -1101,7 +1113,12 @@ NATIVE(linear_cce_forward) {
 NATIVE(linear_cce_backward) {
   const Tensor &in = x.tensor(0), &w = x.tensor(1), &gl = x.tensor(4), &tg = x.tensor(5), &meta = x.tensor(6);
   const Tensor* bias = x.t(2);
+  const Tensor& lse = x.tensor(3);
+  one_device("linear_cross_entropy", in, {&lse, &gl, &meta});
   const flb200_linear_cce_desc d = linear_cce_desc(in, w, bias, tg, x.n32(7), x.n32(8));
+  if (lse.numel() != d.rows || lse.scalar_type() != ScalarType::Float || meta.numel() != 2 ||
+      meta.scalar_type() != ScalarType::Int)
+    value_error("linear_cross_entropy: lse or the counts do not belong to these tensors");
   if (gl.numel() != (d.reduction == FLB200_REDUCE_NONE ? d.rows : 1) || gl.scalar_type() != ScalarType::Float)
     value_error("linear_cross_entropy: the loss's gradient must be float32 and of the loss's shape");
   Tensor gx, gw, gb;
@@ -1109,7 +1126,7 @@ NATIVE(linear_cce_backward) {
   if (x.b(10)) gw = empty(w.sizes(), x.b(12) ? ScalarType::Float : w.scalar_type(), w);
   if (x.b(11)) gb = floats(d.classes, in);
   Workspace ws(flb200_linear_cce_workspace_bytes(&d, P(in), P(w), 1), in);
-  check(unlocked(flb200_linear_cce_backward, &d, P(in), P(w), Pf(bias), Pf(x.t(3)), Pf(&gl),
+  check(unlocked(flb200_linear_cce_backward, &d, P(in), P(w), Pf(bias), Pf(&lse), Pf(&gl),
                  static_cast<const int32_t*>(P(tg)), static_cast<const int32_t*>(P(meta)),
                  gx.defined() ? P(gx) : nullptr, gw.defined() ? P(gw) : nullptr,
                  gw.defined() ? code_of(gw) : d.dtype, gb.defined() ? Pf(&gb) : nullptr, ws.p(), ws.bytes, stream()));
