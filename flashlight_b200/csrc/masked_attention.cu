@@ -798,6 +798,11 @@ join_splits_kernel(const AttnFwdArgs a, long long rows) {
 //     dV += P cols2, dK += dS cols1   or   dQ += dS cols1     (the last 2 D columns)
 // What bounds a unit is its chain from contraction to P and dS to contraction, so as many units are under way as tensor
 // memory holds: three at 64 dimensions (or one in each of two CTAs, see launch_backward), two at 128.
+// dS in f16.  dS is P (dP - D), P about one over the number of keys seen: with the small dO of a training step it falls
+// below 2^-14, where f16 loses bits (750 keys and a dO of 1e-4: dS of 25 of f16's least numbers).  So f16 keeps it times
+// a power of two, 2^shift, which brings the norm of dO to [1, 2) where it is below: of a query's own for dQ, of the
+// call's greatest for dK, whose sums run over queries.  It costs nothing: it goes into the exponent that P is made from
+// (dQ), or into D and a fused product (dK); the sums are multiplied by 2^-shift in fp32.
 // Nothing is added across CTAs: the result does not depend on their order.  The price is that S and dP are made
 // twice, 7 contractions where sums in device memory need 5; those would cost 4 bytes a value per key block.
 template <int D, int UNITS>
@@ -811,13 +816,23 @@ struct BwdSmem {
   static constexpr int kColumns = kUnits * 2 * 64 * 16;  // two buffers of lse, D and interval per query column
   static constexpr int kTotal = 2 * kTile + 2 * kStages * kTile + kColumns + 1024 + 256;
 };
+constexpr int kTops = 1152;  // CTAs that leave a maximum, at most; a multiple of 128
 struct AttnBwdArgs {
   AttnShape s;
   const float* lse;   // [batch][heads][q_len]
   const float* dsum;  // the same of D
+  const float* shift; // the same of dQ's shift (f16)
+  const float* tops;  // [top_count <= kTops]: their greatest is that of |dO|^2 (f16)
+  int top_count;
   OutTensor dq, dk, dv;
   int kv_ctas;        // the first of the grid: dK and dV
 };
+
+// The power of two that brings a norm below one, given squared, to [1, 2); 0 for others and what is not a number.
+__device__ __forceinline__ float shift_of(float norm2) {
+  if (!(norm2 > 0.f && norm2 < 1.f)) return 0.f;
+  return (float)(-(((int)(__float_as_uint(norm2) >> 23) - 127) >> 1));
+}
 
 template <int D, int UNITS, typename T, bool CAP, bool BIAS, bool KV>
 __device__ __forceinline__ void
@@ -827,6 +842,7 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
   constexpr int kStages = SM::kStages, kTile = SM::kTile, kUnits = SM::kUnits;
   constexpr uint32_t kSums = SM::kTmem - 2 * D;  // first column of the sums
   constexpr int kByFma = gradient_by_fma(D, CAP);
+  constexpr bool kShift = std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) char smem_raw[];
   char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   char *sR1 = base, *sR2 = base + kTile, *sC1 = base + 2 * kTile, *sC2 = sC1 + kStages * kTile;
@@ -837,6 +853,7 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
            *bar_p = bar_s + kUnits, *bar_a = bar_p + kUnits;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_a + 1);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* tops = reinterpret_cast<float*>(tmem_slot + 2);  // [4 kUnits] of the call's greatest |dO|^2, a warp's part each
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int nq = blocks_of(a.s.q_len), nk = blocks_of(a.s.k_len), off = a.s.k_len - a.s.q_len;
@@ -886,6 +903,18 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
     }
   }
   if (warp == SM::kMma) tmem_alloc(tmem_slot, SM::kTmem);
+  if (kShift && KV && warp < 4 * kUnits) {
+    float top = 0.f;
+#pragma unroll
+    for (int k = warp; k < kTops / 128; k += 4 * kUnits) {
+      const int at = 32 * k + lane;
+      if (4 * at >= a.top_count) continue;
+      const float4 x = reinterpret_cast<const float4*>(a.tops)[at];
+      top = fmaxf(top, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)));
+    }
+    top = warp_max(top);
+    if (lane == 0) tops[warp] = top;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -962,10 +991,22 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
       return l == -INFINITY ? INFINITY : l * kLog2e;
     };
     float my_lse = INFINITY, my_d = 0.f, slope = 0.f;
+    float shift = 0.f, up = 1.f;  // up: 2^shift, of all columns (KV)
+    if (kShift && KV && total > 0) {
+      float top = tops[0];
+#pragma unroll
+      for (int at = 1; at < 4 * kUnits; ++at) top = fmaxf(top, tops[at]);
+      shift = shift_of(top);
+      up = exp2f(shift);
+    }
     int2 seen = make_int2(0, 0);
     if (!KV && mine < a.s.q_len) {
       my_lse = lse_of(rows0 + mine);
       my_d = a.dsum[rows0 + mine];
+      if (kShift) {
+        shift = a.shift[rows0 + mine];
+        my_lse -= shift;
+      }
       seen = a.s.mask.row(batch, mine);
     }
     if (BIAS && !KV) slope = a.s.slopes[head] * kLog2e;
@@ -977,7 +1018,7 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
       if (tid < 64 && q < a.s.q_len) {
         const long long at = rows0 + (long long)hq * a.s.q_len + q;
         c.seen = a.s.mask.row(batch, q);
-        c.ld = make_float2(lse_of(at), a.dsum[at]);
+        c.ld = make_float2(lse_of(at), kShift ? up * a.dsum[at] : a.dsum[at]);
       }
       return c;
     };
@@ -1052,7 +1093,10 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
               p0 = ex2(p0);
               p1 = ex2(p1);
             }
-            F2 d = pair(__uint_as_float(dr[e]), __uint_as_float(dr[e + 1])) + (KV ? pair(-x.y, -x.w) : pair(-my_d));
+            const F2 less_d = KV ? pair(-x.y, -x.w) : pair(-my_d);
+            F2 d = pair(__uint_as_float(dr[e]), __uint_as_float(dr[e + 1]));
+            if constexpr (kShift && KV) d = fused(d, pair(up), less_d);
+            else d = d + less_d;
             d = d * pair(p0, p1);
             if (CAP) d = d * flat;
             unpair(d, d0, d1);
@@ -1088,6 +1132,7 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
     if (total > 0) wait(bar_a, 0, 6);
     // dV and dK, 2 D columns of sums, or dQ, the last D: 16 columns at a time, in turn
     const int rows = KV ? a.s.k_len : a.s.q_len;
+    const float down = kShift ? a.s.scale * exp2f(-shift) : a.s.scale;
 #pragma unroll 1
     for (int c = (KV ? 0 : D) + 16 * w; c < 2 * D; c += 16 * kUnits) {
       uint32_t o[16];
@@ -1102,7 +1147,7 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
       }
       if (mine < rows)
         store16_of<T>(KV ? (c < D ? a.dv : a.dk) : a.dq, batch, mine, head, c & (D - 1), a.s.head_dim, o,
-                      c < D ? 1.f : a.s.scale, nullptr);
+                      c < D ? 1.f : down, nullptr);
     }
   }
   if (*failed)
@@ -1129,39 +1174,69 @@ masked_backward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     backward_body<D, UNITS, T, CAP, BIAS, false>(map_q, map_k, map_v, map_do, a, blockIdx.x - a.kv_ctas);
 }
 
-// D = rowsum(dO * (O + rest)): LANES lanes per row, one 16-byte load of each.  Results in [batch][heads][q_len].
+// D = rowsum(dO * (O + rest)): LANES lanes per row, one 16-byte load of each.  Results in [batch][heads][q_len].  In f16
+// also each row's shift, and each CTA's greatest |dO|^2 of its rows; there CTAs take several runs of rows each, so that
+// these are few.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256)
 masked_dsum_kernel(const OutTensor o, const T* __restrict__ rest, const OutTensor go, float* __restrict__ dsum,
-                   long long rows, int q_len, int heads, int head_dim) {
+                   float* __restrict__ shift, float* __restrict__ tops, long long rows, int q_len, int heads,
+                   int head_dim) {
+  constexpr bool kShift = std::is_same<T, __half>::value;
   chain_begin();
-  const long long t = blockIdx.x * 256LL + threadIdx.x, r = t / LANES;
-  const int c = 8 * (int)(t % LANES);
-  float acc = 0.f;
-  long long bt = 0, b = 0;
-  int h = 0;
-  if (r < rows) {
-    bt = r / heads;
-    h = (int)(r - bt * heads);
-    b = bt / q_len;
-    if (c < head_dim) {
-      const long long i = bt - b * q_len;
-      float x[8], g[8];
-      unpack16(load16(static_cast<const T*>(o.p) + b * o.batch + i * o.row + h * o.head + c), x);
-      unpack16(load16(static_cast<const T*>(go.p) + b * go.batch + i * go.row + h * go.head + c), g);
-      if (rest) {
-        float y[8];
-        unpack16(load16(rest + r * head_dim + c), y);
+  const int c = 8 * (int)(threadIdx.x % LANES);
+  float top = 0.f;
+  for (long long r0 = blockIdx.x * (256LL / LANES); r0 < rows; r0 += gridDim.x * (256LL / LANES)) {
+    const long long r = r0 + threadIdx.x / LANES;
+    float acc = 0.f, norm2 = 0.f;
+    long long bt = 0, b = 0;
+    int h = 0;
+    if (r < rows) {
+      bt = r / heads;
+      h = (int)(r - bt * heads);
+      b = bt / q_len;
+      if (c < head_dim) {
+        const long long i = bt - b * q_len;
+        float x[8], g[8];
+        unpack16(load16(static_cast<const T*>(o.p) + b * o.batch + i * o.row + h * o.head + c), x);
+        unpack16(load16(static_cast<const T*>(go.p) + b * go.batch + i * go.row + h * go.head + c), g);
+        if (rest) {
+          float y[8];
+          unpack16(load16(rest + r * head_dim + c), y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] += y[e];
+          for (int e = 0; e < 8; ++e) x[e] += y[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc = fmaf(x[e], g[e], acc);
+        if (kShift)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) norm2 = fmaf(g[e], g[e], norm2);
       }
+    }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc = fmaf(x[e], g[e], acc);
+    for (int k = 1; k < LANES; k <<= 1) {
+      acc += __shfl_xor_sync(0xffffffffu, acc, k);
+      if (kShift) norm2 += __shfl_xor_sync(0xffffffffu, norm2, k);
+    }
+    if (r < rows && c == 0) {
+      const long long at = (b * heads + h) * q_len + bt - b * q_len;
+      dsum[at] = acc;
+      if (kShift) shift[at] = shift_of(norm2);
+    }
+    if (kShift && norm2 < INFINITY) top = fmaxf(top, norm2);
+  }
+  if constexpr (kShift) {
+    __shared__ float met[8];
+    top = warp_max(top);
+    if ((threadIdx.x & 31) == 0) met[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+      for (int w = 1; w < 8; ++w) top = fmaxf(top, met[w]);
+      tops[blockIdx.x] = top;
+      for (unsigned at = gridDim.x; blockIdx.x == 0 && at % 4 != 0; ++at) tops[at] = 0.f;  // (read four at a time)
     }
   }
-#pragma unroll
-  for (int k = 1; k < LANES; k <<= 1) acc += __shfl_xor_sync(0xffffffffu, acc, k);
-  if (r < rows && c == 0) dsum[(b * heads + h) * q_len + bt - b * q_len] = acc;
 }
 
 // ------------------------------------------------------------------------------------------ host
@@ -1196,6 +1271,12 @@ int splits_of(const flb200_attention_desc* d) {
   const long long ctas = d->batch * d->heads * blocks_of(d->q_len), places = 2LL * device_info().sm_count;
   const long long s = std::min(places / ctas, (long long)blocks_of(d->k_len) / 4);
   return s < 2 ? 1 : (int)s;
+}
+// CTAs of the gradient's first pass.  In f16, where each leaves a maximum that every CTA of dK and dV reads, about as
+// many as the SMs hold at once.
+unsigned dsum_ctas(const flb200_attention_desc* d) {
+  const long long lanes = d->head_dim <= 64 ? 8 : 16, ctas = (d->batch * d->heads * d->q_len * lanes + 255) / 256;
+  return (unsigned)(d->dtype == FLB200_F16 ? std::min(ctas, (long long)kTops) : ctas);
 }
 int padded_dim(const flb200_attention_desc* d) { return d->head_dim <= 64 ? 64 : 128; }
 
@@ -1373,8 +1454,9 @@ int flb200_masked_attention_forward(const flb200_attention_desc* d, const flb200
 }
 
 size_t flb200_masked_attention_backward_workspace_bytes(const flb200_attention_desc* d) {
-  return !d || d->batch < 1 || d->heads < 1 || d->q_len < 1 ? 0
-                                                            : (size_t)(d->batch * d->heads * d->q_len) * sizeof(float);
+  if (!d || d->batch < 1 || d->heads < 1 || d->q_len < 1) return 0;
+  const size_t rows = (size_t)(d->batch * d->heads * d->q_len);
+  return d->dtype == FLB200_F16 ? 2 * round16(rows * sizeof(float)) + kTops * sizeof(float) : rows * sizeof(float);
 }
 
 int flb200_masked_attention_backward(const flb200_attention_desc* d, const flb200_head_tensor* q,
@@ -1402,11 +1484,13 @@ int flb200_masked_attention_backward(const flb200_attention_desc* d, const flb20
   if (int rc = head_map(&mg, *grad_out, d->batch, d->heads, d->q_len, d->head_dim, operand)) return rc;
   float* dsum = static_cast<float*>(workspace);
   const long long rows = d->batch * d->heads * d->q_len;
+  float* shift = dsum + round16(rows * sizeof(float)) / sizeof(float);  // (these two in f16)
+  float* tops = shift + round16(rows * sizeof(float)) / sizeof(float);
   const auto row_sums = [&](auto type, auto lanes) {
     using T = decltype(type);
-    launch_chained(masked_dsum_kernel<T, decltype(lanes)::value>, (unsigned)((rows * lanes + 255) / 256), 256, 0, st,
-                   out_of(*out, d->head_dim), static_cast<const T*>(rest), out_of(*grad_out, d->head_dim), dsum, rows,
-                   (int)d->q_len, (int)d->heads, (int)d->head_dim);
+    launch_chained(masked_dsum_kernel<T, decltype(lanes)::value>, dsum_ctas(d), 256, 0, st,
+                   out_of(*out, d->head_dim), static_cast<const T*>(rest), out_of(*grad_out, d->head_dim), dsum,
+                   shift, tops, rows, (int)d->q_len, (int)d->heads, (int)d->head_dim);
   };
   const auto by_lanes = [&](auto type) {
     if (d->head_dim <= 64) row_sums(type, std::integral_constant<int, 8>{});
@@ -1419,6 +1503,9 @@ int flb200_masked_attention_backward(const flb200_attention_desc* d, const flb20
   a.s = shape_of(d, slopes, mask);
   a.lse = lse;
   a.dsum = dsum;
+  a.shift = shift;
+  a.tops = tops;
+  a.top_count = (int)dsum_ctas(d);
   a.dq = out_of(*grad_q, d->head_dim);
   a.dk = out_of(*grad_k, d->head_dim);
   a.dv = out_of(*grad_v, d->head_dim);

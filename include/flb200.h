@@ -611,8 +611,9 @@ int flb200_attention_mask(int64_t batch, int64_t q_len, int64_t k_len, int causa
  * mask leaves; softcap 0: s = scale q.k - ..., slopes (fp32 [heads], a constant: it takes no gradient) may be NULL.
  * Query head h reads key head h / (heads / kv_heads).  FLB200_F16 or FLB200_BF16, head_dim a multiple of 8 up to
  * 128 (flb200_masked_attention_supported; else FLB200_UNSUPPORTED); scores, statistics and sums are fp32, the
- * probabilities and the scores' gradient are rounded to the tensors' type as operands (in f16 the latter must
- * stay below 65504, as the gradients themselves must).  Tensors by strides in
+ * probabilities and the scores' gradient are rounded to the tensors' type as operands.  In f16 the latter must stay
+ * below 65504, as the gradients themselves must; where the norm of a row of grad_out is below one (for grad_k: of
+ * every row), it is kept times the power of two that brings the norm to [1, 2).  Tensors by strides in
  * elements, each a multiple of 8, data 16-byte aligned: element (b, t, h, d) at b*batch + t*row + h*head + d.
  * What the mask leaves out has weight zero whatever its score, but the products multiply values by those zeros.  So
  * where some query of a block of 128 sees a part of a block of 128 keys, all of that block's v must be finite, or the
