@@ -47,7 +47,10 @@ class AdamWOptimizer:
     the step: p -= lr * (m^ / (sqrt(v^) + epsilon) + weight_decay * p).  One launch for all parameters
     (functions.adamw_step).  state_bits=8 keeps m and sqrt(v) as e4m3 bytes with a scale per 256 elements:
     2 bytes per element instead of 8.  Parameters without a gradient are passed over; the step's number counts
-    all calls.  The states of all parameters lie one after another in `first` and `second`."""
+    all calls that made a step.  The states of all parameters lie one after another in `first` and `second`.  The
+    step's number, the rate and the addresses are arguments of the launch: a step captured in a CUDA graph repeats one
+    number's corrections of the moments and one rate with every replay, so capture the model's step without it, or
+    capture it again."""
 
     def __init__(self, parameters: List[Variable], learning_rate: float, beta1: float = 0.9,
                  beta2: float = 0.999, epsilon: float = 1e-8, weight_decay: float = 0.0, state_bits: int = 32):

@@ -515,7 +515,8 @@ int flb200_sgd_step(void* param, void* grad, void* velocity, int64_t n, float lr
  *   the block's largest magnitude / 448; a root above zero has a code above zero.  The step uses m and v
  *   before they are rounded.  An infinite gradient leaves NaN in its whole block's states.
  * Tensors aligned to eight elements (of f32: 32 bytes) are read in whole vectors, others one by one.  Empty
- * tensors are passed over.  Everything is read on the host during the call: `tensors` may be reused after it. */
+ * tensors are passed over.  Everything is read on the host during the call: `tensors` may be reused after it, and a
+ * call captured in a graph repeats its own step number, rate and addresses. */
 enum { FLB200_ADAMW_BLOCK = 256 };
 typedef struct flb200_adamw_tensor {
   void* param;
