@@ -251,15 +251,15 @@ __device__ __forceinline__ void exp2_by_fma(F2 z, float& a, float& b) {
                __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u));
   unpair(p, a, b);
 }
-// One pair of a row's exponentials in this many is made so, the others by the special function unit (0: all).  At 64
-// dimensions that unit is the busiest, at 128 the tensor pipe, but with a cap, which takes two more of it a score.
-// us with none, one in eight, in four, in two:
-//   16 heads of 8192 causal positions of 64, forward 195, 190, 182, 206; gradient 524, 505, 519, 552
-//   12 in documents of 3000 with a distance bias, forward 106, 101, 110, 122
-//   16 of 8192 of 128, forward 246, 258, 268, 276
-//   2 x 1500, a cap, 16 of 128, forward 57, 49, 53, 60; gradient 150, 128, 142, 144
-constexpr int forward_by_fma(int D, bool cap, bool bias) { return cap ? 8 : D == 64 ? (bias ? 8 : 4) : 0; }
-constexpr int gradient_by_fma(int D, bool cap) { return D == 64 || cap ? 8 : 0; }
+// One pair of a row's exponentials in this many is made so in the forward pass, the others by the special function unit
+// (0: all).  At 64 dimensions that unit is the busiest, but with a distance bias, whose arithmetic is the FMA pipe's; at
+// 128 it is the tensor pipe.  us with none, one in eight, in four, in two:
+//   16 heads of 8192 causal positions of 64, forward 199, 193, 183, 206; gradient 514, 538, 528, 571
+//   16 heads of 2 x 4096 of 64, a cap, forward 239, 234, 232; gradient 556, 550, 551
+//   12 in documents of 3000 of 64 with a distance bias, forward 105, 107, 106; gradient 201, 202, 208
+//   16 of 8192 of 128, forward 266, 266, 267, 284; 2 x 1500, a cap, 54, 53, 53; gradient 127, 126, 126
+// The gradient, whose chains leave that unit idle half the time, makes none so.
+constexpr int forward_by_fma(int D, bool bias) { return D == 64 && !bias ? 4 : 0; }
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (std::is_same<T, __half>::value) {
@@ -450,7 +450,7 @@ masked_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   using SM = FwdSmem<D>;
   constexpr int kStages = SM::kStages, kTile = SM::kTile;
   constexpr bool kApart = D == 64;                  // P beside S
-  constexpr int kByFma = forward_by_fma(D, CAP, BIAS);
+  constexpr int kByFma = forward_by_fma(D, BIAS);
   constexpr uint32_t kP = kApart ? 192 : 0;         // its first column
   extern __shared__ __align__(1024) char smem_raw[];
   char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -841,7 +841,6 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
   using SM = BwdSmem<D, UNITS>;
   constexpr int kStages = SM::kStages, kTile = SM::kTile, kUnits = SM::kUnits;
   constexpr uint32_t kSums = SM::kTmem - 2 * D;  // first column of the sums
-  constexpr int kByFma = gradient_by_fma(D, CAP);
   constexpr bool kShift = std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) char smem_raw[];
   char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -1086,13 +1085,9 @@ backward_body(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensor
               z = fused(z, pair(a.s.to_log2), less);
             }
             float p0, p1, d0, d1;
-            if (kByFma > 0 && !decltype(tested)::value && (e / 2) % (kByFma + !kByFma) == 0) {
-              exp2_by_fma(z, p0, p1);
-            } else {
-              unpair(z, p0, p1);
-              p0 = ex2(p0);
-              p1 = ex2(p1);
-            }
+            unpair(z, p0, p1);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
             const F2 less_d = KV ? pair(-x.y, -x.w) : pair(-my_d);
             F2 d = pair(__uint_as_float(dr[e]), __uint_as_float(dr[e + 1]));
             if constexpr (kShift && KV) d = fused(d, pair(up), less_d);
