@@ -1351,8 +1351,8 @@ int launch_backward(const flb200_attention_desc* d, const CUtensorMap& mq, const
   if constexpr (D == 64) {
     // Short rows are bound by what a CTA does before its first and after its last unit, which a second CTA on the SM
     // fills; long ones by the units under way, of which one CTA holds three and two CTAs one each.  12 heads of 8 x 512,
-    // documents of 128: 28 us with two CTAs, 37 with one; 16 of 2 x 4096 316 and 308, in documents of 1000
-    // 145 and 156; 16 of 8192 562 and 521.
+    // documents of 128: 27 us with two CTAs, 37 with one; 16 of 2 x 4096 315 and 301, in documents of 1000
+    // 144 and 155; 16 of 8192 570 and 516, in documents of 1000 149 and 155.
     if (d->k_len <= 4096) return launch_backward_as<D, 1, T, CAP, BIAS>(d, mq, mk, mv, mg, a, st);
     return launch_backward_as<D, 3, T, CAP, BIAS>(d, mq, mk, mv, mg, a, st);
   } else {
