@@ -801,8 +801,9 @@ join_splits_kernel(const AttnFwdArgs a, long long rows) {
 // dS in f16.  dS is P (dP - D), P about one over the number of keys seen: with the small dO of a training step it falls
 // below 2^-14, where f16 loses bits (750 keys and a dO of 1e-4: dS of 25 of f16's least numbers).  So f16 keeps it times
 // a power of two, 2^shift, which brings the norm of dO to [1, 2) where it is below: of a query's own for dQ, of the
-// call's greatest for dK, whose sums run over queries.  It costs nothing: it goes into the exponent that P is made from
-// (dQ), or into D and a fused product (dK); the sums are multiplied by 2^-shift in fp32.
+// call's greatest for dK, whose sums run over queries.  It goes into the exponent that P is made from (dQ), or into D and a
+// fused product (dK); the sums are multiplied by 2^-shift in fp32.  A load a row and the maximum at a CTA's start are 1 to
+// 4 % of the gradient's time (16 heads of 8192 of 64: 560 -> 568 us; 8 x 512, 12 heads: 39 -> 41).
 // Nothing is added across CTAs: the result does not depend on their order.  The price is that S and dP are made
 // twice, 7 contractions where sums in device memory need 5; those would cost 4 bytes a value per key block.
 template <int D, int UNITS>
@@ -1451,7 +1452,7 @@ int flb200_masked_attention_forward(const flb200_attention_desc* d, const flb200
 size_t flb200_masked_attention_backward_workspace_bytes(const flb200_attention_desc* d) {
   if (!d || d->batch < 1 || d->heads < 1 || d->q_len < 1) return 0;
   const size_t rows = (size_t)(d->batch * d->heads * d->q_len);
-  return d->dtype == FLB200_F16 ? 2 * round16(rows * sizeof(float)) + kTops * sizeof(float) : rows * sizeof(float);
+  return (d->dtype == FLB200_F16 ? 2 * rows + 4 + kTops : rows) * sizeof(float);  // (4: tops on 16 bytes)
 }
 
 int flb200_masked_attention_backward(const flb200_attention_desc* d, const flb200_head_tensor* q,
@@ -1461,6 +1462,8 @@ int flb200_masked_attention_backward(const flb200_attention_desc* d, const flb20
                                      const flb200_head_tensor* grad_q, const flb200_head_tensor* grad_k,
                                      const flb200_head_tensor* grad_v, void* workspace, size_t workspace_bytes,
                                      void* stream) {
+  if (reinterpret_cast<uintptr_t>(workspace) & 3)
+    return fail(FLB200_WORKSPACE_TOO_SMALL, "masked_attention_backward: the workspace must be 4-byte aligned");
   if (int rc = check_attention("masked_attention_backward", d)) return rc;
   FLB200_REQUIRE(lse, "masked_attention_backward: null lse");
   FLB200_REQUIRE(!mask || aligned16(mask), "masked_attention_backward: the mask must be 16-byte aligned");
@@ -1479,8 +1482,8 @@ int flb200_masked_attention_backward(const flb200_attention_desc* d, const flb20
   if (int rc = head_map(&mg, *grad_out, d->batch, d->heads, d->q_len, d->head_dim, operand)) return rc;
   float* dsum = static_cast<float*>(workspace);
   const long long rows = d->batch * d->heads * d->q_len;
-  float* shift = dsum + round16(rows * sizeof(float)) / sizeof(float);  // (these two in f16)
-  float* tops = shift + round16(rows * sizeof(float)) / sizeof(float);
+  float* shift = dsum + rows;  // (these two in f16)
+  float* tops = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(shift + rows) + 15) & ~(uintptr_t)15);
   const auto row_sums = [&](auto type, auto lanes) {
     using T = decltype(type);
     launch_chained(masked_dsum_kernel<T, decltype(lanes)::value>, dsum_ctas(d), 256, 0, st,

@@ -638,7 +638,8 @@ typedef struct flb200_head_tensor {
   int64_t batch, row, head; /* strides */
 } flb200_head_tensor;
 int flb200_masked_attention_supported(const flb200_attention_desc* d);
-/* (0 unless there are few queries and many keys, whose blocks are then shared out and joined) */
+/* (0 unless there are few queries and many keys, whose blocks are then shared out and joined.)  Forward's workspace must
+ * be 16-byte aligned, backward's 4-byte aligned; else FLB200_WORKSPACE_TOO_SMALL. */
 size_t flb200_masked_attention_forward_workspace_bytes(const flb200_attention_desc* d);
 int flb200_masked_attention_forward(const flb200_attention_desc* d, const flb200_head_tensor* q,
                                     const flb200_head_tensor* k, const flb200_head_tensor* v,

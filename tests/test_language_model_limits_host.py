@@ -78,3 +78,12 @@ def test_loss_refuses_tensors_of_several_devices(fake):
         bad[i] = there(bad[i])
         with pytest.raises(ValueError, match="one device"):
             F.linear_cross_entropy_backward(*bad[:5], F.CrossEntropyState(bad[5], bad[6], L.REDUCE_MEAN, -1))
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_attention_gradient_refuses_a_workspace_off_4_bytes(off):
+    d = L.AttentionDesc(batch=1, q_len=4, k_len=4, heads=4, kv_heads=2, head_dim=64, scale=1.0, softcap=0.0, dtype=L.F16)
+    t = C.byref(L.HeadTensor(16, 1024, 256, 64))
+    assert L.lib.flb200_masked_attention_backward(C.byref(d), t, t, t, t, None, t, 16, None, None, t, t, t, 4096 + off,
+                                                  1 << 40, None) == L.WORKSPACE_TOO_SMALL
+    assert b"4-byte aligned" in L.lib.flb200_last_error()
